@@ -10,9 +10,28 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("COMPREX_GFX950_LIB") or os.path.join(_HERE, "lib", "libcomprex_gfx950.so")
 CSRC_DIR = os.path.join(_HERE, "csrc")
 
-CX_F32, CX_F64, CX_I32 = 0, 1, 2
+CX_F32, CX_F64, CX_I32, CX_BF16, CX_F16 = 0, 1, 2, 3, 4
 (CX_OK, CX_ERR_INVALID, CX_ERR_SIZE_MISMATCH, CX_ERR_MSG_TOO_LARGE, CX_ERR_CAPACITY, CX_ERR_INDEX,
  CX_ERR_HIP, CX_ERR_INTERNAL, CX_ERR_TOPK) = range(9)
+
+
+class AdamwState(C.Structure):
+    """cx_adamw_state"""
+    _fields_ = [("param_type", C.c_int), ("state_bits", C.c_int), ("params", C.c_void_p), ("masters", C.c_void_p),
+                ("exp_avg", C.c_void_p), ("exp_avg_sq", C.c_void_p), ("exp_avg_scales", C.c_void_p),
+                ("exp_avg_sq_scales", C.c_void_p)]
+
+
+class Grads(C.Structure):
+    """cx_grads"""
+    _fields_ = [("type", C.c_int), ("each", C.c_void_p), ("flat", C.c_void_p)]
+
+
+class AdamwArgs(C.Structure):
+    """cx_adamw_args"""
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("scale", C.c_double), ("step", C.c_longlong), ("d_step", C.c_void_p),
+                ("d_lr", C.c_void_p), ("d_coefs", C.c_void_p), ("n_coefs", C.c_int), ("d_skip", C.c_void_p)]
 
 
 class ComprexError(RuntimeError):
@@ -82,6 +101,13 @@ def lib():
         "cx_ip_reduce": (i, [vp, i, vp, i, C.POINTER(vp), i, i, i]),
         "cx_zero": (i, [vp, i, vp, i]),
         "cx_add_vec": (i, [vp, i, vp, vp, i]),
+        "cx_tensors_create": (i, [C.POINTER(vp), vp, i, vp, C.POINTER(AdamwState)]),
+        "cx_tensors_destroy": (i, [vp]),
+        "cx_grad_norms": (i, [vp, vp, C.POINTER(Grads), C.c_double, C.c_double, i, vp, vp, vp]),
+        "cx_pack": (i, [vp, vp, C.POINTER(Grads), vp, i, C.c_double, vp, vp]),
+        "cx_adamw_step": (i, [vp, vp, C.POINTER(Grads), C.POINTER(AdamwArgs)]),
+        "cx_adamw_states": (i, [vp, vp, i, vp, vp]),
+        "cx_adamw_set_states": (i, [vp, vp, vp, vp]),
         "cx_threshold_apply": (i, [vp, i, vp, vp, vp, i, vp, vp]),
     }
     for name, (res, args) in protos.items():

@@ -1,0 +1,385 @@
+// Many tensors at once: the set itself (cx_tensors_*), the gradients' norms and clip coefficients, and
+// the flat vector that the compressor takes (keras/comprex_optimizer.py:97-133 of the reference does the
+// latter two tensor after tensor).
+#include "cx_tensors.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <memory>
+
+namespace cx {
+
+namespace {
+
+constexpr int kBlock = 256;
+
+__device__ __forceinline__ double wave_sum(double x) {
+    for (int d = 32; d > 0; d >>= 1) x += __shfl_xor(x, d);
+    return x;
+}
+
+// The block's sum, in thread 0.
+template <int BLOCK> __device__ __forceinline__ double block_sum(double x) {
+    __shared__ double part[BLOCK / 64];
+    x = wave_sum(x);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
+    __syncthreads();
+    double s = 0.0;
+    for (int k = 0; k < BLOCK / 64; ++k) s += part[k];
+    return s;
+}
+
+// partial[piece] = sum of g^2.  64 bits: the squares of finite floats do not overflow there.
+template <typename G>
+__global__ __launch_bounds__(kBlock) void squares_kernel(const Chunk* __restrict__ chunks, int first, GradArgs ga,
+                                                         double* __restrict__ partial) {
+    const Chunk c = chunks[first + blockIdx.x];
+    const G* g = grad_of<G>(c, ga);
+    double s = 0.0;
+    if (g) {
+        for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4) {
+            const Vec4<float> x = to_float<G>(load_up_to4(g + i, c.n - i));
+            for (int k = 0; k < 4; ++k) s += (double)x[k] * (double)x[k];
+        }
+    }
+    s = block_sum<kBlock>(s);
+    if (threadIdx.x == 0) partial[first + blockIdx.x] = s;
+}
+
+__device__ __forceinline__ float clip_coef(double norm, double max_norm) {
+    return norm > max_norm ? (float)(max_norm / norm) : 1.0f;
+}
+
+// Block t < count: tensor t's norm; block `count`: that of all, from all pieces' sums in a fixed order.
+__global__ __launch_bounds__(kBlock) void norms_kernel(const double* __restrict__ partial,
+                                                       const int* __restrict__ first_chunk, int count, double scale,
+                                                       double max_norm, int each, float* __restrict__ norms,
+                                                       float* __restrict__ coefs, int* __restrict__ nonfinite) {
+    const int t = blockIdx.x;
+    const int from = t < count ? first_chunk[t] : 0, to = first_chunk[t < count ? t + 1 : count];
+    double s = 0.0;
+    for (int i = from + threadIdx.x; i < to; i += kBlock) s += partial[i];
+    s = block_sum<kBlock>(s);
+    if (threadIdx.x != 0) return;
+    const double norm = sqrt(s) * scale;
+    if (norms) norms[t] = (float)norm;
+    if (coefs && each && t < count) coefs[t] = clip_coef(norm, max_norm);
+    if (coefs && !each && t == count) coefs[0] = clip_coef(norm, max_norm);
+    if (nonfinite && t == count) *nonfinite = s <= 1.7976931348623157e308 ? 0 : 1;
+}
+
+template <typename G>
+__global__ __launch_bounds__(kBlock) void pack_kernel(const Chunk* __restrict__ chunks, int first, GradArgs ga,
+                                                      const float* __restrict__ coefs, int per_tensor, float scale,
+                                                      const int* __restrict__ skip, float* out) {
+    const Chunk c = chunks[first + blockIdx.x];
+    const G* g = grad_of<G>(c, ga);
+    float* to = out + c.flat;
+    if (!g || (skip && *skip)) {
+        for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4) store_up_to4(to + i, Vec4<float>{}, c.n - i);
+        return;
+    }
+    const float f = factor_of(c, coefs, per_tensor, scale);
+    for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4)
+        store_up_to4(to + i, to_float<G>(load_up_to4(g + i, c.n - i)) * f, c.n - i);
+}
+
+// Elements per piece: a multiple of 1024, so that a piece of a tensor begins a block of 8-bit states.
+int chunk_elements(long long total) {
+    long long c = 1024;
+    while (c < 16384 && c * 2048 < total) c *= 2;
+    return (int)c;
+}
+
+struct Span {
+    uintptr_t from, to;
+};
+
+void add_span(std::vector<Span>& spans, const void* p, long long bytes) {
+    if (p && bytes > 0) spans.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + (uintptr_t)bytes});
+}
+
+int element_bytes(int dt) { return dt == CX_F32 ? 4 : 2; }
+
+bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+
+}  // namespace
+
+#define CX_NUM_DISPATCH(dt, CALL)                                                     \
+    switch (dt) {                                                                     \
+        case CX_F32: { using G = Num<CX_F32>::type; CALL; } break;                    \
+        case CX_BF16: { using G = Num<CX_BF16>::type; CALL; } break;                  \
+        default: { using G = Num<CX_F16>::type; CALL; } break;                        \
+    }
+
+int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale, double max_norm, int each,
+                      float* d_norms, float* d_coefs, int* d_nonfinite) {
+    int rc = for_grads(t, g, [&](int first, int n, const GradArgs& a) -> int {
+        CX_NUM_DISPATCH(g->type, (squares_kernel<G><<<n, kBlock, 0, h->stream>>>(t->d_chunks, first, a, t->d_partial)));
+        CX_HIP(hipGetLastError());
+        return CX_OK;
+    });
+    if (rc != CX_OK) return rc;
+    norms_kernel<<<t->count + 1, kBlock, 0, h->stream>>>(t->d_partial, t->d_first_chunk, t->count, std::fabs(scale),
+                                                         max_norm, each, d_norms, d_coefs, d_nonfinite);
+    CX_HIP(hipGetLastError());
+    return CX_OK;
+}
+
+int launch_pack(cx_handle h, cx_tensors t, const cx_grads* g, const float* d_coefs, int n_coefs, float scale,
+                const int* d_skip, float* out) {
+    return for_grads(t, g, [&](int first, int n, const GradArgs& a) -> int {
+        CX_NUM_DISPATCH(g->type, (pack_kernel<G><<<n, kBlock, 0, h->stream>>>(t->d_chunks, first, a, d_coefs,
+                                                                              n_coefs != 1, scale, d_skip, out)));
+        CX_HIP(hipGetLastError());
+        return CX_OK;
+    });
+}
+
+}  // namespace cx
+
+using namespace cx;
+
+namespace {
+
+bool number_type(int dt) { return dt == CX_F32 || dt == CX_BF16 || dt == CX_F16; }
+
+// What every call over a set checks first.
+int check_set(cx_handle h, cx_tensors t, const char* who) {
+    if (!h || !t) return fail(CX_ERR_INVALID, "%s: null handle or set", who);
+    if (h->device != t->device)
+        return fail(CX_ERR_INVALID, "%s: the set lives on device %d, the handle on %d", who, t->device, h->device);
+    return CX_OK;
+}
+
+int check_grads(cx_tensors t, const cx_grads* g, const char* who) {
+    if (!g || !number_type(g->type)) return fail(CX_ERR_INVALID, "%s: gradients are fp32, bf16 or fp16", who);
+    if (t->total > 0 && !g->each == !g->flat)
+        return fail(CX_ERR_INVALID, "%s: needs either the tensors' gradients or the flat vector", who);
+    const int bytes = element_bytes(g->type);
+    if (g->flat && !aligned_to(g->flat, bytes)) return fail(CX_ERR_INVALID, "%s: misaligned gradient", who);
+    if (g->each)
+        for (int k = 0; k < t->count; ++k)
+            if (!aligned_to(g->each[k], bytes)) return fail(CX_ERR_INVALID, "%s: misaligned gradient %d", who, k);
+    return CX_OK;
+}
+
+int check_coefs(cx_tensors t, const float* d_coefs, int n_coefs, const char* who) {
+    if (n_coefs != 0 && n_coefs != 1 && n_coefs != t->count)
+        return fail(CX_ERR_SIZE_MISMATCH, "%s: %d coefficients for %d tensors", who, n_coefs, t->count);
+    if (n_coefs != 0 && !d_coefs) return fail(CX_ERR_INVALID, "%s: null coefficients", who);
+    return CX_OK;
+}
+
+}  // namespace
+
+static int create_tensors(cx_tensors* out, cx_handle h, int count, const long long* sizes, const cx_adamw_state* state) {
+    if (!out) return fail(CX_ERR_INVALID, "cx_tensors_create: null output");
+    *out = nullptr;
+    if (!h || count < 0 || (count > 0 && !sizes)) return fail(CX_ERR_INVALID, "cx_tensors_create: bad arguments");
+    long long total = 0;
+    for (int k = 0; k < count; ++k) {
+        if (sizes[k] < 0 || sizes[k] > (1ll << 40) || (total += sizes[k]) > (1ll << 40))
+            return fail(CX_ERR_INVALID, "cx_tensors_create: tensor %d has a size of %lld", k, sizes[k]);
+    }
+    if (state) {
+        if (!number_type(state->param_type))
+            return fail(CX_ERR_INVALID, "cx_tensors_create: parameters are fp32, bf16 or fp16");
+        if (state->state_bits != 32 && state->state_bits != 8)
+            return fail(CX_ERR_INVALID, "cx_tensors_create: states have 32 or 8 bits, not %d", state->state_bits);
+        if (state->masters && state->param_type == CX_F32)
+            return fail(CX_ERR_INVALID, "cx_tensors_create: fp32 parameters have no masters");
+        const bool small = state->state_bits == 8;
+        if (count > 0 && (!state->params || !state->exp_avg || !state->exp_avg_sq ||
+                          small != (state->exp_avg_scales != nullptr) || small != (state->exp_avg_sq_scales != nullptr)))
+            return fail(CX_ERR_INVALID, "cx_tensors_create: a list of the state is missing or superfluous");
+        std::vector<Span> spans;
+        for (int k = 0; k < count; ++k) {
+            const long long n = sizes[k], blocks = (n + CX_STATE_BLOCK - 1) / CX_STATE_BLOCK;
+            if (n == 0) continue;
+            const int pb = element_bytes(state->param_type), sb = small ? 1 : 4;
+            if (!state->params[k] || !state->exp_avg[k] || !state->exp_avg_sq[k] ||
+                (state->masters && !state->masters[k]) ||
+                (small && (!state->exp_avg_scales[k] || !state->exp_avg_sq_scales[k])))
+                return fail(CX_ERR_INVALID, "cx_tensors_create: tensor %d has a null buffer", k);
+            if (!aligned_to(state->params[k], pb) || !aligned_to(state->exp_avg[k], sb) ||
+                !aligned_to(state->exp_avg_sq[k], sb) || (state->masters && !aligned_to(state->masters[k], 4)) ||
+                (small && (!aligned_to(state->exp_avg_scales[k], 4) || !aligned_to(state->exp_avg_sq_scales[k], 4))))
+                return fail(CX_ERR_INVALID, "cx_tensors_create: tensor %d has a misaligned buffer", k);
+            add_span(spans, state->params[k], n * pb);
+            add_span(spans, state->exp_avg[k], n * sb);
+            add_span(spans, state->exp_avg_sq[k], n * sb);
+            if (state->masters) add_span(spans, state->masters[k], n * 4);
+            if (small) {
+                add_span(spans, state->exp_avg_scales[k], blocks * 4);
+                add_span(spans, state->exp_avg_sq_scales[k], blocks * 4);
+            }
+        }
+        std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].from < spans[i - 1].to)
+                return fail(CX_ERR_INVALID, "cx_tensors_create: two of the buffers overlap (a tensor given twice?)");
+    }
+
+    DeviceScope on(h->device);
+    CX_HIP(on.error);
+    std::unique_ptr<cx_tensors_s, int (*)(cx_tensors)> owner(new cx_tensors_s(), cx_tensors_destroy);
+    cx_tensors t = owner.get();
+    t->device = h->device;
+    t->count = count;
+    t->total = total;
+    t->adamw = state != nullptr;
+    if (state) {
+        t->param_type = state->param_type;
+        t->state_bits = state->state_bits;
+        t->masters = state->masters != nullptr;
+    }
+    const int step = chunk_elements(total);
+    std::vector<Chunk> chunks;
+    long long flat = 0;
+    for (int k = 0; k < count; ++k) {
+        t->sizes.push_back(sizes[k]);
+        t->flat.push_back(flat);
+        t->first_chunk.push_back((int)chunks.size());
+        for (long long at = 0; at < sizes[k]; at += step) {
+            Chunk c = {};
+            c.at = at;
+            c.flat = flat + at;
+            c.tensor = k;
+            c.n = (int)std::min<long long>(step, sizes[k] - at);
+            if (state) {
+                const long long pb = element_bytes(state->param_type), sb = state->state_bits / 8;
+                c.param = static_cast<char*>(state->params[k]) + at * pb;
+                c.master = state->masters ? state->masters[k] + at : nullptr;
+                c.m = static_cast<char*>(state->exp_avg[k]) + at * sb;
+                c.v = static_cast<char*>(state->exp_avg_sq[k]) + at * sb;
+                if (state->state_bits == 8) {
+                    c.m_scale = state->exp_avg_scales[k] + at / CX_STATE_BLOCK;
+                    c.v_scale = state->exp_avg_sq_scales[k] + at / CX_STATE_BLOCK;
+                }
+            }
+            chunks.push_back(c);
+        }
+        flat += sizes[k];
+    }
+    t->first_chunk.push_back((int)chunks.size());
+    t->chunks = (int)chunks.size();
+    const size_t nc = chunks.empty() ? 1 : chunks.size();
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&t->d_chunks), nc * sizeof(Chunk));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_first_chunk), (count + 1) * sizeof(int));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_partial), nc * sizeof(double));
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_rates), 256);
+    if (e == hipSuccess && !chunks.empty())
+        e = hipMemcpyAsync(t->d_chunks, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice, h->stream);
+    if (e == hipSuccess)
+        e = hipMemcpyAsync(t->d_first_chunk, t->first_chunk.data(), (count + 1) * sizeof(int), hipMemcpyHostToDevice,
+                           h->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(h->stream);
+    if (e != hipSuccess) return fail(CX_ERR_HIP, "cx_tensors_create: %s", hipGetErrorString(e));
+    *out = owner.release();
+    return CX_OK;
+}
+
+extern "C" {
+
+int cx_tensors_create(cx_tensors* out, cx_handle h, int count, const long long* sizes, const cx_adamw_state* state) {
+    try {
+        return create_tensors(out, h, count, sizes, state);
+    } catch (const std::exception& e) {  // the host tables did not fit
+        return fail(CX_ERR_INVALID, "cx_tensors_create: %s", e.what());
+    }
+}
+
+int cx_tensors_destroy(cx_tensors t) {
+    if (!t) return CX_OK;
+    DeviceScope on(t->device);
+    if (t->d_chunks) (void)hipFree(t->d_chunks);  // waits for the device
+    if (t->d_first_chunk) (void)hipFree(t->d_first_chunk);
+    if (t->d_partial) (void)hipFree(t->d_partial);
+    if (t->d_rates) (void)hipFree(t->d_rates);
+    delete t;
+    return CX_OK;
+}
+
+int cx_grad_norms(cx_handle h, cx_tensors t, const cx_grads* grads, double scale, double max_norm, int each,
+                  float* d_norms, float* d_coefs, int* d_nonfinite) {
+    int rc = check_set(h, t, "cx_grad_norms");
+    if (rc == CX_OK) rc = check_grads(t, grads, "cx_grad_norms");
+    if (rc != CX_OK) return rc;
+    if (!(max_norm > 0.0)) return fail(CX_ERR_INVALID, "cx_grad_norms: max_norm must be above 0");
+    if (!std::isfinite(scale)) return fail(CX_ERR_INVALID, "cx_grad_norms: scale must be finite");
+    DeviceScope on(t->device);
+    CX_HIP(on.error);
+    return launch_grad_norms(h, t, grads, scale, max_norm, each != 0, d_norms, d_coefs, d_nonfinite);
+}
+
+int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coefs, int n_coefs, double scale,
+            const int* d_skip, float* out) {
+    int rc = check_set(h, t, "cx_pack");
+    if (rc == CX_OK) rc = check_grads(t, grads, "cx_pack");
+    if (rc == CX_OK) rc = check_coefs(t, d_coefs, n_coefs, "cx_pack");
+    if (rc != CX_OK) return rc;
+    if ((!out && t->total > 0) || !aligned_to(out, 4)) return fail(CX_ERR_INVALID, "cx_pack: null or misaligned output");
+    const char *lo = reinterpret_cast<const char*>(out), *hi = lo + t->total * 4;
+    const int bytes = element_bytes(grads->type);
+    for (int k = 0; k < t->count; ++k) {
+        if (t->sizes[k] == 0) continue;  // (of an empty set neither form of the gradients need be there)
+        const char* g = grads->flat ? static_cast<const char*>(grads->flat) + t->flat[k] * bytes
+                                    : static_cast<const char*>(grads->each[k]);
+        if (!g || g >= hi || g + t->sizes[k] * bytes <= lo) continue;
+        if (grads->type != CX_F32 || g != lo + t->flat[k] * 4)
+            return fail(CX_ERR_INVALID, "cx_pack: the output overlaps gradient %d", k);
+    }
+    DeviceScope on(t->device);
+    CX_HIP(on.error);
+    return launch_pack(h, t, grads, n_coefs ? d_coefs : nullptr, n_coefs, (float)scale, d_skip, out);
+}
+
+int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* a) {
+    int rc = check_set(h, t, "cx_adamw_step");
+    if (rc == CX_OK) rc = check_grads(t, grads, "cx_adamw_step");
+    if (rc == CX_OK && !a) rc = fail(CX_ERR_INVALID, "cx_adamw_step: null arguments");
+    if (rc == CX_OK) rc = check_coefs(t, a->d_coefs, a->n_coefs, "cx_adamw_step");
+    if (rc != CX_OK) return rc;
+    if (!t->adamw) return fail(CX_ERR_INVALID, "cx_adamw_step: the set was made without a state");
+    if (!a->d_lr && !(a->lr >= 0.0 && std::isfinite(a->lr)))
+        return fail(CX_ERR_INVALID, "cx_adamw_step: the learning rate must be finite and not negative");
+    if (!(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0))
+        return fail(CX_ERR_INVALID, "cx_adamw_step: the betas must lie in [0, 1)");
+    if (!(a->eps > 0.0 && std::isfinite(a->eps) && (float)a->eps >= 1e-20f))
+        return fail(CX_ERR_INVALID, "cx_adamw_step: eps must be finite and at least 1e-20");
+    if (!(a->weight_decay >= 0.0 && std::isfinite(a->weight_decay)))
+        return fail(CX_ERR_INVALID, "cx_adamw_step: the weight decay must be finite and not negative");
+    if (!std::isfinite(a->scale)) return fail(CX_ERR_INVALID, "cx_adamw_step: scale must be finite");
+    if (!a->d_step && a->step < 1) return fail(CX_ERR_INVALID, "cx_adamw_step: steps count from 1");
+    DeviceScope on(t->device);
+    CX_HIP(on.error);
+    return launch_adamw(h, t, grads, a);
+}
+
+int cx_adamw_states(cx_handle h, cx_tensors t, cx_dtype dt, void* d_exp_avg, void* d_exp_avg_sq) {
+    const int rc = check_set(h, t, "cx_adamw_states");
+    if (rc != CX_OK) return rc;
+    if (!t->adamw || t->state_bits != 8) return fail(CX_ERR_INVALID, "cx_adamw_states: the set has no 8-bit states");
+    if (!number_type(dt)) return fail(CX_ERR_INVALID, "cx_adamw_states: values are fp32, bf16 or fp16");
+    if (t->total > 0 && (!d_exp_avg || !d_exp_avg_sq || !aligned_to(d_exp_avg, element_bytes(dt)) ||
+                         !aligned_to(d_exp_avg_sq, element_bytes(dt))))
+        return fail(CX_ERR_INVALID, "cx_adamw_states: null or misaligned output");
+    DeviceScope on(t->device);
+    CX_HIP(on.error);
+    return launch_adamw_states(h, t, dt, d_exp_avg, d_exp_avg_sq);
+}
+
+int cx_adamw_set_states(cx_handle h, cx_tensors t, const float* d_exp_avg, const float* d_exp_avg_sq) {
+    const int rc = check_set(h, t, "cx_adamw_set_states");
+    if (rc != CX_OK) return rc;
+    if (!t->adamw || t->state_bits != 8) return fail(CX_ERR_INVALID, "cx_adamw_set_states: the set has no 8-bit states");
+    if (t->total > 0 && (!d_exp_avg || !d_exp_avg_sq || !aligned_to(d_exp_avg, 4) || !aligned_to(d_exp_avg_sq, 4)))
+        return fail(CX_ERR_INVALID, "cx_adamw_set_states: null or misaligned input");
+    DeviceScope on(t->device);
+    CX_HIP(on.error);
+    return launch_adamw_set_states(h, t, d_exp_avg, d_exp_avg_sq);
+}
+
+}  // extern "C"

@@ -10,9 +10,11 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import CX_F32, CX_F64, CX_I32, ComprexError, check  # noqa: F401
+from ._lib import CX_BF16, CX_F16, CX_F32, CX_F64, CX_I32, ComprexError, check  # noqa: F401
 
 _DT = {torch.float32: CX_F32, torch.float64: CX_F64, torch.int32: CX_I32}
+# parameters and gradients of the operators over many tensors
+_NUM = {torch.float32: CX_F32, torch.bfloat16: CX_BF16, torch.float16: CX_F16}
 _CT = {torch.float32: C.c_float, torch.float64: C.c_double, torch.int32: C.c_int}
 
 
@@ -34,6 +36,158 @@ def _dt(t):
     return _DT[t.dtype]
 
 
+def _invalid(text, *args, code=_lib.CX_ERR_INVALID):
+    return ComprexError(code, text % args)
+
+
+def _addresses(tensors):
+    """Host array of the tensors' addresses (None: no tensor)."""
+    return (C.c_void_p * len(tensors))(*[None if t is None else t.data_ptr() for t in tensors])
+
+
+class TensorSet:
+    """The tensors of a training step (cx_tensors): how many elements each has, for `Handle.grad_norms`
+    and `Handle.pack`.  Made once per model and kept; belongs on one stream at a time, and a graph captured
+    with it needs it alive."""
+
+    def __init__(self, handle, sizes):
+        self._make(handle, [int(n) for n in sizes], None)
+
+    def _make(self, handle, sizes, state):
+        self.lib, self.sizes, self.device = handle.lib, sizes, handle.device
+        self.total = sum(sizes)
+        self._t = C.c_void_p()
+        if any(n < 0 or n >= 1 << 62 for n in sizes):
+            raise _invalid("a tensor cannot have %d elements", min(sizes) if min(sizes) < 0 else max(sizes))
+        check(self.lib.cx_tensors_create(C.byref(self._t), handle._h, len(sizes), (C.c_longlong * len(sizes))(*sizes),
+                                         state))
+
+    def close(self):
+        if getattr(self, "_t", None):
+            self.lib.cx_tensors_destroy(self._t)
+            self._t = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _grads(self, grads):
+        """cx_grads of a list (an entry per tensor, None: no gradient) or of a flat vector, checked."""
+        if isinstance(grads, torch.Tensor):
+            if grads.dim() != 1 or grads.numel() != self.total:
+                raise _invalid("a flat gradient has %d elements in one dimension, got %s", self.total,
+                               tuple(grads.shape), code=_lib.CX_ERR_SIZE_MISMATCH)
+            if grads.dtype not in _NUM or grads.device != self.device or not grads.is_contiguous():
+                raise _invalid("a flat gradient is a contiguous fp32, bf16 or fp16 tensor on %s", self.device)
+            return _lib.Grads(_NUM[grads.dtype], None, grads.data_ptr())
+        if len(grads) != len(self.sizes):
+            raise _invalid("%d gradients for %d tensors", len(grads), len(self.sizes), code=_lib.CX_ERR_SIZE_MISMATCH)
+        dtype, device, addresses = None, self.device, []
+        for g, n in zip(grads, self.sizes):
+            if g is None:
+                addresses.append(None)
+                continue
+            if dtype is None:
+                dtype = g.dtype
+            if g.numel() != n:
+                raise _invalid("gradient of %d elements for a tensor of %d", g.numel(), n, code=_lib.CX_ERR_SIZE_MISMATCH)
+            if g.dtype != dtype or g.device != device or not g.is_contiguous():
+                raise _invalid("gradients are contiguous tensors of one type on %s", device)
+            addresses.append(g.data_ptr())
+        if dtype is None:
+            dtype = torch.float32
+        elif dtype not in _NUM:
+            raise _invalid("gradients are fp32, bf16 or fp16, not %s", dtype)
+        each = (C.c_void_p * len(addresses))(*addresses)
+        found = _lib.Grads(_NUM[dtype], C.cast(each, C.c_void_p), None)
+        found.kept = each
+        return found
+
+    def _coefs(self, coefs):
+        if coefs is None:
+            return None, 0
+        if coefs.dtype != torch.float32 or coefs.device != self.device or not coefs.is_contiguous():
+            raise _invalid("coefficients are a contiguous fp32 tensor on %s", self.device)
+        return coefs.data_ptr(), coefs.numel()
+
+    def _one(self, t, dtype, what):
+        """Address of a one-element device tensor, None for None."""
+        if t is None:
+            return None
+        if t.dtype != dtype or t.device != self.device or t.numel() != 1:
+            raise _invalid("%s is one element of %s on %s", what, dtype, self.device)
+        return t.data_ptr()
+
+    def _vector(self, t, dtype, what):
+        """A given vector of all elements, checked, or a new one."""
+        if t is None:
+            return torch.empty(self.total, dtype=dtype, device=self.device)
+        if t.dtype != dtype or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
+            raise _invalid("%s is a contiguous vector of %s on %s", what, dtype, self.device)
+        if t.numel() != self.total:
+            raise _invalid("%s has %d elements, not %d", what, self.total, t.numel(), code=_lib.CX_ERR_SIZE_MISMATCH)
+        return t
+
+
+class AdamWSet(TensorSet):
+    """A TensorSet with what `Handle.adamw_step` updates: lists with a tensor per parameter.  `params`: fp32, bf16
+    or fp16; `masters`: None, or the fp32 weights that bf16 or fp16 parameters are rounded from.  Moments in 32 bits:
+    `exp_avg` and `exp_avg_sq` fp32.  Moments in 8 bits: `exp_avg` float8_e4m3fn, `exp_avg_sq` uint8 codes
+    (include/comprex_gfx950.h says what they stand for), and fp32 scales, one for every `BLOCK` elements of a
+    tensor; `AdamWSet.zeros8` makes them.  The tensors are kept, and updated where they are: one that moves
+    needs a new set."""
+
+    BLOCK = 256
+
+    def __init__(self, handle, params, exp_avg, exp_avg_sq, masters=None, exp_avg_scales=None, exp_avg_sq_scales=None):
+        lists = [params, exp_avg, exp_avg_sq, masters, exp_avg_scales, exp_avg_sq_scales]
+        lists = [None if x is None else list(x) for x in lists]
+        params, exp_avg, exp_avg_sq, masters, exp_avg_scales, exp_avg_sq_scales = lists
+        small = exp_avg_scales is not None
+        if small != (exp_avg_sq_scales is not None):
+            raise _invalid("8-bit moments need the scales of both")
+        sizes = [p.numel() for p in params]
+        if params and params[0].dtype not in _NUM:
+            raise _invalid("parameters are fp32, bf16 or fp16, not %s", params[0].dtype)
+        dtype = params[0].dtype if params else torch.float32
+        if not params:
+            lists[3] = None  # nothing to have masters of
+        elif masters is not None and dtype == torch.float32:
+            raise _invalid("fp32 parameters have no masters")
+        blocks = [-(-n // self.BLOCK) for n in sizes]
+        f32 = torch.float32
+        wanted = [("params", dtype, sizes), ("exp_avg", torch.float8_e4m3fn if small else f32, sizes),
+                  ("exp_avg_sq", torch.uint8 if small else f32, sizes), ("masters", f32, sizes),
+                  ("exp_avg_scales", f32, blocks), ("exp_avg_sq_scales", f32, blocks)]
+        for got, (name, dt, ns) in zip(lists, wanted):
+            if got is None:
+                continue
+            if len(got) != len(sizes):
+                raise _invalid("%d %s for %d parameters", len(got), name, len(sizes), code=_lib.CX_ERR_SIZE_MISMATCH)
+            for t, n in zip(got, ns):
+                if t.numel() != n:
+                    raise _invalid("%s has %d elements where %d belong", name, t.numel(), n,
+                                   code=_lib.CX_ERR_SIZE_MISMATCH)
+                if t.dtype != dt or t.device != handle.device or not t.is_contiguous():
+                    raise _invalid("%s are contiguous tensors of %s on %s", name, dt, handle.device)
+        self.kept = lists
+        self.state_bits = 8 if small else 32
+        arrays = [None if x is None else _addresses(x) for x in lists]
+        at = [None if a is None else C.cast(a, C.c_void_p) for a in arrays]
+        self._make(handle, sizes, C.byref(_lib.AdamwState(_NUM[dtype], self.state_bits, at[0], at[3], at[1], at[2], at[4],
+                                                          at[5])))
+
+    @classmethod
+    def zeros8(cls, param):
+        """(exp_avg, exp_avg_sq, exp_avg_scales, exp_avg_sq_scales) of a parameter at the start of training."""
+        n = param.numel()
+        return (torch.zeros(n, dtype=torch.uint8, device=param.device).view(torch.float8_e4m3fn),
+                torch.zeros(n, dtype=torch.uint8, device=param.device),
+                torch.zeros(-(-n // cls.BLOCK), device=param.device), torch.zeros(-(-n // cls.BLOCK), device=param.device))
+
+
 class Handle:
     """One compressor clone's scratch + stream (cx_create / cx_destroy)."""
 
@@ -43,6 +197,7 @@ class Handle:
         if stream is None:
             stream = torch.cuda.current_stream()
         self.stream = stream
+        self.device = torch.device("cuda", torch.cuda.current_device())
         check(self.lib.cx_create(C.byref(self._h), C.c_void_p(stream.cuda_stream)))
 
     def close(self):
@@ -219,6 +374,68 @@ class Handle:
         check(self.lib.cx_threshold_apply(self._h, _dt(vec), _p(high), _p(low), _p(vec), vec.numel(),
                                           C.byref(hthr), None))
         return (high, low) if split else high
+
+
+    # ---- many tensors ------------------------------------------------------
+    def grad_norms(self, tensors, grads, max_norm=None, each=False, scale=1.0, norms=None, coefs=None, nonfinite=None):
+        """Norms of `scale` times the gradients of a TensorSet and their clip coefficients: (norms, coefs,
+        nonfinite), on the device.  norms[t] is tensor t's, norms[-1] that of all; coefs: one, from the norm of
+        all, or with `each` one for every tensor from its own (max_norm None clips nothing); nonfinite: int32, 1
+        where a gradient holds an infinity or NaN.  `grads`: a list (None: no gradient) or the flat vector."""
+        count = len(tensors.sizes)
+        g = tensors._grads(grads)
+        out = []
+        for t, n, dt, what in ((norms, count + 1, torch.float32, "norms"), (coefs, count if each else 1, torch.float32, "coefs"),
+                               (nonfinite, 1, torch.int32, "nonfinite")):
+            if t is None:
+                t = torch.empty(n, dtype=dt, device=tensors.device)
+            elif t.dtype != dt or t.device != tensors.device or t.numel() != n or not t.is_contiguous():
+                raise _invalid("%s: %d contiguous elements of %s on %s", what, n, dt, tensors.device)
+            out.append(t)
+        check(self.lib.cx_grad_norms(self._h, tensors._t, g, scale, float("inf") if max_norm is None else max_norm,
+                                     1 if each else 0, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr()))
+        return tuple(out)
+
+    def pack(self, tensors, grads, out=None, coefs=None, scale=1.0, skip=None):
+        """The gradients of a TensorSet, times coefs (one, or one per tensor) and scale, back to back in a flat
+        fp32 vector: what the compressor and the allreduce schedules take.  `skip` (int32, e.g. grad_norms'
+        nonfinite) other than 0: all zeros."""
+        g = tensors._grads(grads)
+        out = tensors._vector(out, torch.float32, "the flat vector")
+        at, n = tensors._coefs(coefs)
+        check(self.lib.cx_pack(self._h, tensors._t, g, at, n, scale, tensors._one(skip, torch.int32, "skip"),
+                               out.data_ptr()))
+        return out
+
+    def adamw_step(self, tensors, grads, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, coefs=None, scale=1.0,
+                   skip=None):
+        """One AdamW step on an AdamWSet with the gradients times coefs and scale (cx_adamw_step).  `grads`: a
+        list (None: leave this tensor alone) or the flat vector; `step`: which step this is, from 1, or an int32
+        device tensor that the call advances; `lr`: a number or an fp32 device tensor; `skip` (int32) other than
+        0: nothing changes."""
+        g = tensors._grads(grads)
+        on_device = isinstance(step, torch.Tensor)
+        d_lr = isinstance(lr, torch.Tensor)
+        at, n = tensors._coefs(coefs)
+        check(self.lib.cx_adamw_step(self._h, tensors._t, g, _lib.AdamwArgs(
+            0.0 if d_lr else lr, betas[0], betas[1], eps, weight_decay, scale, 0 if on_device else step,
+            tensors._one(step, torch.int32, "step") if on_device else None,
+            tensors._one(lr, torch.float32, "lr") if d_lr else None, at, n, tensors._one(skip, torch.int32, "skip"))))
+
+    def adamw_states(self, tensors, dtype=torch.float32, exp_avg=None, exp_avg_sq=None):
+        """What the 8-bit moments of an AdamWSet stand for: (exp_avg, exp_avg_sq), flat vectors of `dtype`."""
+        if dtype not in _NUM:
+            raise _invalid("values are fp32, bf16 or fp16, not %s", dtype)
+        m, v = tensors._vector(exp_avg, dtype, "exp_avg"), tensors._vector(exp_avg_sq, dtype, "exp_avg_sq")
+        check(self.lib.cx_adamw_states(self._h, tensors._t, _NUM[dtype], m.data_ptr(), v.data_ptr()))
+        return m, v
+
+    def adamw_set_states(self, tensors, exp_avg, exp_avg_sq):
+        """Sets the 8-bit moments of an AdamWSet from flat fp32 vectors (exp_avg_sq: not below 0)."""
+        if exp_avg is None or exp_avg_sq is None:
+            raise _invalid("needs the values of both moments")
+        check(self.lib.cx_adamw_set_states(self._h, tensors._t, tensors._vector(exp_avg, torch.float32, "exp_avg").data_ptr(),
+                                           tensors._vector(exp_avg_sq, torch.float32, "exp_avg_sq").data_ptr()))
 
 
 def message_to_numpy(msg, nbytes):

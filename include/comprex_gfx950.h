@@ -36,7 +36,9 @@ extern "C" {
 
 typedef struct cx_handle_s* cx_handle;
 
-typedef enum { CX_F32 = 0, CX_F64 = 1, CX_I32 = 2 } cx_dtype;
+/* CX_BF16 and CX_F16 are types of parameters and gradients (the entry points over many tensors below);
+ * the codecs, thresholds and reductions take the first three. */
+typedef enum { CX_F32 = 0, CX_F64 = 1, CX_I32 = 2, CX_BF16 = 3, CX_F16 = 4 } cx_dtype;
 
 typedef enum {
     CX_OK = 0,
@@ -295,6 +297,99 @@ int cx_add_vec(cx_handle h, cx_dtype dt, void* data, const void* rests, int n);
  * out = |in| >= thr ? in : 0, and apply_split (:30-50) when `low` is not NULL. */
 int cx_threshold_apply(cx_handle h, cx_dtype dt, void* high, void* low, const void* in, int n,
                        const void* thr_host, const void* d_thr);
+
+/* ---- many tensors: clipping, packing, the AdamW step ------------------------ */
+/* What a training step does around the exchange, over all tensors of a model at once: the gradients'
+ * norms and clip coefficients, the flat vector the compressor takes, the weights' update.  The reference
+ * does the first two and a momentum update tensor after tensor in Keras (keras/comprex_optimizer.py:97-163);
+ * AdamW has no counterpart there.  Nothing here reads a device value on the host, waits or allocates
+ * (cx_tensors_create apart), so a step may be captured in a HIP graph. */
+
+/* The tensors of such a step: their sizes, the pieces the kernels walk, what AdamW updates, and the
+ * scratch of the norms.  All calls that use one set belong on one stream at a time; a graph that was
+ * captured with it needs it alive. */
+typedef struct cx_tensors_s* cx_tensors;
+
+/* What cx_adamw_step updates: HOST arrays of `count` device pointers each (an entry of an empty tensor may
+ * be NULL).  Elements lie back to back; no pointer needs more than its element type's alignment.
+ *
+ * state_bits 32: exp_avg and exp_avg_sq are floats; the two arrays of scales are NULL.
+ * state_bits 8: one byte per element and one float scale per block of CX_STATE_BLOCK elements of a tensor
+ * (the last block may be shorter).  exp_avg: e4m3 codes (OCP, 448 the largest) of m * 448 / M, M = the
+ * block's largest |m|, scale M / 448.  exp_avg_sq: floats of 5 exponent and 3 mantissa bits without a sign
+ * (code 8 e + f stands for 2^(e-1) (1 + f/8), for f / 8 where e = 0), in units that give the block's
+ * largest value V the code 255, scale V; a value above 0 never becomes code 0.  Both are rounded to
+ * nearest.  A block whose M (or V) is below 2^-100 is stored as zeros with scale 0.  Elements that are not
+ * finite count in no maximum: their exp_avg is stored as NaN and they leave their block's others alone.
+ * Bytes and scales that are zero stand for zero moments: how training begins. */
+enum { CX_STATE_BLOCK = 256 };
+typedef struct {
+    cx_dtype param_type;       /* CX_F32, CX_BF16 or CX_F16 */
+    int state_bits;            /* 32 or 8 */
+    void* const* params;       /* param_type */
+    float* const* masters;     /* NULL, or the 32-bit weights that `params` are rounded from */
+    void* const* exp_avg;
+    void* const* exp_avg_sq;
+    float* const* exp_avg_scales;
+    float* const* exp_avg_sq_scales;
+} cx_adamw_state;
+
+/* `sizes`: host array of element counts (0 allowed).  state == NULL: for cx_grad_norms and cx_pack only.
+ * Refuses (CX_ERR_INVALID) buffers of `state` that overlap.  Waits for the handle's stream. */
+int cx_tensors_create(cx_tensors* out, cx_handle h, int count, const long long* sizes, const cx_adamw_state* state);
+int cx_tensors_destroy(cx_tensors t);
+
+/* The gradients of a set's tensors, in the set's order: one flat vector (`flat`, the tensors back to back:
+ * what cx_pack writes and the exchange sums), or a HOST array of device pointers (`each`, read during the
+ * call; a NULL entry = this tensor has no gradient).  Exactly one of the two is given. */
+typedef struct {
+    cx_dtype type;             /* CX_F32, CX_BF16 or CX_F16 */
+    const void* const* each;
+    const void* flat;
+} cx_grads;
+
+/* d_norms[t] = |scale| * sqrt(sum of the squares of tensor t), d_norms[count] = that of all tensors
+ * together; sums in 64 bits, so no finite gradient overflows, in an order that is always the same.
+ * Clip coefficients, norm > max_norm ? max_norm / norm : 1: each == 0: d_coefs[0] from the norm of all
+ * (what the gradients share), each != 0: d_coefs[t] from each tensor's own (tf.clip_by_norm,
+ * keras/comprex_optimizer.py:97-133).  max_norm > 0; infinity clips nothing.  *d_nonfinite = 1 when a
+ * gradient holds an infinity or NaN, else 0 (cx_pack and cx_adamw_step take it as d_skip).  d_norms,
+ * d_coefs and d_nonfinite may each be NULL.  A tensor without a gradient has norm 0. */
+int cx_grad_norms(cx_handle h, cx_tensors t, const cx_grads* grads, double scale, double max_norm, int each,
+                  float* d_norms, float* d_coefs, int* d_nonfinite);
+
+/* out[off_t + i] = grads_t[i] * (coef_t * scale), the tensors back to back in `out` (fp32, as many elements as
+ * the set has): the gradient vector that cx_ip_write_step, ComprEx::writeRemote and the allreduce schedules
+ * take (the reference's blob, keras/comprex_optimizer.py:97-124).  n_coefs: 0 (1 for all), 1 or the set's
+ * count.  A tensor without a gradient gives zeros.  *d_skip != 0 (d_skip may be NULL) makes all of `out`
+ * zero: a gradient that is not finite would stay in the error-feedback residual for good.  `out` may be the
+ * flat fp32 gradient itself and overlaps the gradients in no other way (CX_ERR_INVALID). */
+int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coefs, int n_coefs, double scale,
+            const int* d_skip, float* out);
+
+/* One AdamW step on every tensor of the set that has a gradient, with g = grads * (coef * scale), w the
+ * master where there is one and the parameter otherwise:
+ *     m = beta1 m + (1 - beta1) g            v = beta2 v + (1 - beta2) g^2
+ *     w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * in 32 bits; the parameter is w rounded once, 8-bit states are m and v rounded after w took them.
+ * step >= 1 counts this step.  With d_step (device int) the count lives on the device: the call adds 1 to
+ * it and uses the result; `step` is ignored.  d_lr (device float) replaces lr.  *d_skip != 0 leaves
+ * everything as it is, *d_step too. */
+typedef struct {
+    double lr, beta1, beta2, eps, weight_decay, scale;
+    long long step;
+    int* d_step;
+    const float* d_lr;
+    const float* d_coefs;
+    int n_coefs;               /* 0, 1 or the set's count */
+    const int* d_skip;
+} cx_adamw_args;
+int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* args);
+
+/* The values that the 8-bit states of a set stand for, all tensors back to back (dt: CX_F32, CX_BF16 or
+ * CX_F16), and back: states from values (fp32).  For checkpoints that hold 32 bits. */
+int cx_adamw_states(cx_handle h, cx_tensors t, cx_dtype dt, void* d_exp_avg, void* d_exp_avg_sq);
+int cx_adamw_set_states(cx_handle h, cx_tensors t, const float* d_exp_avg, const float* d_exp_avg_sq);
 
 /* ---- the reference's C ABI (float only) ------------------------------------- */
 /* src/GPI_C.cpp:41-73.  One process stands for `ranks` simulated ranks that exchange
