@@ -4,24 +4,63 @@
 
 #include "cx_common.hpp"
 
+#include <type_traits>
 #include <vector>
 
 namespace cx {
 
-// One workgroup's piece of one tensor.  The addresses are those of the piece's first element; a kernel
-// reads one Chunk with scalar loads and needs no other table.
-struct alignas(16) Chunk {
-    long long at;      // first element within its tensor
-    long long flat;    // first element within the flat vector of all tensors
-    int tensor;
-    int n;             // elements
+// One tensor.  A kernel reads one entry with scalar loads.
+struct alignas(16) Tensor {
+    long long n;          // elements
+    long long flat;       // first element within the flat vector of all tensors
+    int first_fine;       // first piece in each of the two divisions below
+    int first_coarse;
     void* param;
-    float* master;     // nullptr: none
-    void* m;           // float or codes
+    float* master;        // nullptr: none
+    void* m;              // float or codes
     void* v;
-    float* m_scale;    // 8-bit states only: the scale of the piece's first block
+    float* m_scale;       // 8-bit states only
     float* v_scale;
 };
+
+// The tensors are cut into pieces, one workgroup's work each; a tensor's last piece may be shorter.  `owner`
+// says which tensor a piece belongs to (4 bytes a piece, and the tensors' table stays in the caches).
+// kFine: everything that reads and writes.  Pieces of one load per stream and lane: all workgroups in flight
+// then walk through each buffer as one narrow front.  fp32 step on 25.6 M elements: 122 us with 1024 elements
+// a piece, 128 with 2048, 141 with 4096, 151 with 16384 (loops over the piece), 159 with 65536.
+// kCoarse: the sums of squares, which want few partial sums.
+enum { kFine = 0, kCoarse = 1 };
+struct Pieces {
+    const Tensor* tensors;
+    const int* owner;
+    int step;             // elements of a piece
+    int first;            // first piece of the launch
+};
+struct Piece {
+    Tensor t;
+    int tensor;
+    long long at;         // first element within the tensor
+    int n;                // elements
+};
+
+// The launch's pieces, dealt out so that each of the 8 XCDs (workgroup b runs on XCD b mod 8) takes 32 in a
+// row: fp32 step on 64 Mi elements 352 us dealt out one by one, 339 / 333 us with 4 / 16 in a row, 366 us with
+// an eighth of the whole each.
+constexpr int kXcds = 8, kRun = 32;
+__device__ __forceinline__ int dealt(int b, int n) {
+    constexpr int round = kXcds * kRun;
+    return b < n / round * round ? b / round * round + b % kXcds * kRun + b % round / kXcds : b;
+}
+
+template <int WHICH> __device__ __forceinline__ Piece piece_of(const Pieces& ps) {
+    Piece c;
+    const int id = ps.first + dealt(blockIdx.x, gridDim.x);
+    c.tensor = __builtin_amdgcn_readfirstlane(ps.owner[id]);
+    c.t = ps.tensors[c.tensor];
+    c.at = (long long)(id - (WHICH == kFine ? c.t.first_fine : c.t.first_coarse)) * ps.step;
+    c.n = (int)min((long long)ps.step, c.t.n - c.at);
+    return c;
+}
 
 // A launch's gradients: one flat vector, or the addresses of up to kGradsPerLaunch tensors.  They travel as
 // kernel arguments, because gradients move between steps where parameters stay: no upload to wait for or to
@@ -40,33 +79,43 @@ template <> struct Num<CX_F16> { using type = _Float16; };
 
 template <typename E> using Vec4 = E __attribute__((ext_vector_type(4)));
 
-// Four elements at any address that is aligned to one: gfx950's vector loads and stores take it.
-template <typename E>
+// Four elements at any address that is aligned to one: gfx950's vector loads and stores take it.  The
+// addresses come out of a table, so the compiler has to be told that they are global memory.  Past the caches
+// (nontemporal) unless `KEEP`: a step touches everything once (fp32 step, 64 Mi elements in pieces of 2048: 355 us,
+// plain loads and stores 358 us, 25.6 M elements 128 and 147 us).
+template <bool KEEP = false, typename E>
 __device__ __forceinline__ Vec4<E> load4(const E* p) {
     typedef Vec4<E> V __attribute__((aligned(sizeof(E))));
-    return *reinterpret_cast<const V*>(p);
+    auto* g = (const __attribute__((address_space(1))) V*)p;
+    if constexpr (KEEP) return *g;
+    else return __builtin_nontemporal_load(g);
 }
 template <typename E>
 __device__ __forceinline__ void store4(E* p, Vec4<E> x) {
     typedef Vec4<E> V __attribute__((aligned(sizeof(E))));
-    *reinterpret_cast<V*>(p) = x;
+    __builtin_nontemporal_store(x, (__attribute__((address_space(1))) V*)p);
 }
-// The first `k` (1..4) of them, zeros for the rest.
-template <typename E>
+template <typename E> __device__ __forceinline__ __attribute__((address_space(1))) E* global(E* p) {
+    return (__attribute__((address_space(1))) E*)p;
+}
+// The first `k` of them, zeros for the rest.  FULL: all four, without asking.
+template <bool FULL = false, bool KEEP = false, typename E>
 __device__ __forceinline__ Vec4<E> load_up_to4(const E* p, int k) {
-    if (k >= 4) return load4(p);
+    if (FULL || k >= 4) return load4<KEEP>(p);
+    const auto* g = global(p);
     Vec4<E> x = {};
-    if (k > 0) x[0] = p[0];
-    if (k > 1) x[1] = p[1];
-    if (k > 2) x[2] = p[2];
+    if (k > 0) x[0] = g[0];
+    if (k > 1) x[1] = g[1];
+    if (k > 2) x[2] = g[2];
     return x;
 }
-template <typename E>
+template <bool FULL = false, typename E>
 __device__ __forceinline__ void store_up_to4(E* p, Vec4<E> x, int k) {
-    if (k >= 4) return store4(p, x);
-    if (k > 0) p[0] = x[0];
-    if (k > 1) p[1] = x[1];
-    if (k > 2) p[2] = x[2];
+    if (FULL || k >= 4) return store4(p, x);
+    auto* g = global(p);
+    if (k > 0) g[0] = x[0];
+    if (k > 1) g[1] = x[1];
+    if (k > 2) g[2] = x[2];
 }
 template <typename E> __device__ __forceinline__ Vec4<float> to_float(Vec4<E> x) {
     return __builtin_convertvector(x, Vec4<float>);
@@ -76,14 +125,22 @@ template <typename E> __device__ __forceinline__ Vec4<E> from_float(Vec4<float> 
 }
 
 // The gradient of a piece, nullptr where its tensor has none.
-template <typename G> __device__ __forceinline__ const G* grad_of(const Chunk& c, const GradArgs& g) {
-    if (g.flat) return static_cast<const G*>(g.flat) + c.flat;
+template <typename G> __device__ __forceinline__ const G* grad_of(const Piece& c, const GradArgs& g) {
+    if (g.flat) return static_cast<const G*>(g.flat) + c.t.flat + c.at;
     const G* p = static_cast<const G*>(g.each[c.tensor - g.first]);
     return p ? p + c.at : nullptr;
 }
 
+// Calls body with true_type for a whole fine piece (no lane asks how many elements it has) and false_type for
+// a tensor's last one.
+constexpr int kFineStep = 1024;
+template <typename F> __device__ __forceinline__ void by_length(const Piece& c, F&& body) {
+    if (c.n == kFineStep) body(std::true_type{});
+    else body(std::false_type{});
+}
+
 // coef * scale of a piece's tensor
-__device__ __forceinline__ float factor_of(const Chunk& c, const float* coefs, int per_tensor, float scale) {
+__device__ __forceinline__ float factor_of(const Piece& c, const float* coefs, int per_tensor, float scale) {
     return coefs ? coefs[per_tensor ? c.tensor : 0] * scale : scale;
 }
 
@@ -109,35 +166,44 @@ struct DeviceScope {
 struct cx_tensors_s {
     int device = 0;
     int count = 0;
-    int chunks = 0;
     long long total = 0;
     std::vector<long long> sizes, flat;     // per tensor; flat: its first element in the flat vector
-    std::vector<int> first_chunk;           // count + 1
+    struct Division {
+        int step = 0;                       // elements of a piece
+        int pieces = 0;
+        std::vector<int> first;             // count + 1
+        int* d_owner = nullptr;
+        int* d_first = nullptr;             // `first` on the device
+    } cut[2];                               // kFine, kCoarse
     bool adamw = false;
     int param_type = 0, state_bits = 0;
     bool masters = false;
     // device
-    cx::Chunk* d_chunks = nullptr;
-    int* d_first_chunk = nullptr;           // count + 1
-    double* d_partial = nullptr;            // per piece: sum of the gradient's squares
+    cx::Tensor* d_tensors = nullptr;
+    double* d_partial = nullptr;            // per coarse piece: sum of the gradient's squares
     float* d_rates = nullptr;               // what a device-side step count gives (AdamwRates)
+
+    cx::Pieces pieces(int which, int from = 0) const {
+        return {d_tensors, cut[which].d_owner, cut[which].step, from};
+    }
 };
 
 namespace cx {
 
-// Calls `launch(first_chunk, n_chunks, args)` for as many tensors at a time as one launch's arguments hold.
-template <typename F> int for_grads(cx_tensors t, const cx_grads* g, F&& launch) {
+// Calls `launch(pieces, number of pieces, args)` for as many tensors at a time as one launch's arguments hold.
+template <typename F> int for_grads(cx_tensors t, const cx_grads* g, int which, F&& launch) {
+    const auto& cut = t->cut[which];
     GradArgs a;
     a.flat = g->flat;
     a.first = 0;
-    if (t->chunks == 0) return CX_OK;
-    if (g->flat) return launch(0, t->chunks, a);
+    if (cut.pieces == 0) return CX_OK;
+    if (g->flat) return launch(t->pieces(which), cut.pieces, a);
     for (int first = 0; first < t->count; first += kGradsPerLaunch) {
         const int last = first + kGradsPerLaunch < t->count ? first + kGradsPerLaunch : t->count;
         a.first = first;
         for (int k = first; k < last; ++k) a.each[k - first] = g->each[k];
-        const int from = t->first_chunk[first], n = t->first_chunk[last] - from;
-        const int rc = n ? launch(from, n, a) : CX_OK;
+        const int from = cut.first[first], n = cut.first[last] - from;
+        const int rc = n ? launch(t->pieces(which, from), n, a) : CX_OK;
         if (rc != CX_OK) return rc;
     }
     return CX_OK;

@@ -15,7 +15,7 @@ namespace cx {
 
 namespace {
 
-constexpr int kBlock = 256;
+constexpr int kBlock = 256;   // 4 elements a lane: a piece of 1024
 
 // What depends on the step's count.
 struct AdamwRates {
@@ -57,6 +57,7 @@ __device__ __forceinline__ void moments(Vec4<float> g, const AdamwArgs& a, Vec4<
 
 __device__ __forceinline__ Vec4<float> weights(Vec4<float> w, Vec4<float> m, Vec4<float> v, const AdamwArgs& a,
                                                const AdamwRates& r) {
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float below = __builtin_fmaf(__builtin_sqrtf(v[k]), r.v_unit, a.eps);
         w[k] -= __builtin_fmaf(r.decay, w[k], r.step * (m[k] / below));
@@ -64,60 +65,62 @@ __device__ __forceinline__ Vec4<float> weights(Vec4<float> w, Vec4<float> m, Vec
     return w;
 }
 
+// One piece a workgroup, four elements a lane: everything is asked for before anything is used.
 template <typename P, typename G, bool MASTER>
-__global__ __launch_bounds__(kBlock) void adamw32_kernel(const Chunk* __restrict__ chunks, int first, GradArgs ga,
-                                                         AdamwArgs a) {
-    const Chunk c = chunks[first + blockIdx.x];
+__global__ __launch_bounds__(kBlock) void adamw32_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
+    const Piece c = piece_of<kFine>(ps);
     const G* g = grad_of<G>(c, ga);
     if (!g || (a.skip && *a.skip)) return;
     const AdamwRates r = a.device_rates ? *a.device_rates : a.rates;
     const float f = factor_of(c, a.coefs, a.per_tensor, a.scale);
-    P* p = static_cast<P*>(c.param);
-    float *pm = static_cast<float*>(c.m), *pv = static_cast<float*>(c.v);
-    for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4) {
-        const int k = c.n - i;
-        const Vec4<float> x = to_float<G>(load_up_to4(g + i, k)) * f;
-        Vec4<float> m = load_up_to4(pm + i, k), v = load_up_to4(pv + i, k);
+    P* p = static_cast<P*>(c.t.param) + c.at;
+    float *pm = static_cast<float*>(c.t.m) + c.at, *pv = static_cast<float*>(c.t.v) + c.at, *pw = c.t.master + c.at;
+    const int i = threadIdx.x * 4, k = c.n - i;
+    if (k <= 0) return;
+    by_length(c, [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const Vec4<G> gx = load_up_to4<FULL>(g + i, k);
+        Vec4<float> m = load_up_to4<FULL>(pm + i, k), v = load_up_to4<FULL>(pv + i, k);
         Vec4<float> w;
-        if constexpr (MASTER) w = load_up_to4(c.master + i, k);
-        else w = to_float<P>(load_up_to4(p + i, k));
-        moments(x, a, m, v);
+        if constexpr (MASTER) w = load_up_to4<FULL>(pw + i, k);
+        else w = to_float<P>(load_up_to4<FULL>(p + i, k));
+        moments(to_float<G>(gx) * f, a, m, v);
         w = weights(w, m, v, a, r);
-        store_up_to4(pm + i, m, k);
-        store_up_to4(pv + i, v, k);
-        if constexpr (MASTER) store_up_to4(c.master + i, w, k);
-        store_up_to4(p + i, from_float<P>(w), k);
-    }
+        store_up_to4<FULL>(pm + i, m, k);
+        store_up_to4<FULL>(pv + i, v, k);
+        if constexpr (MASTER) store_up_to4<FULL>(pw + i, w, k);
+        store_up_to4<FULL>(p + i, from_float<P>(w), k);
+    });
 }
 
 // ---- 8-bit moments ---------------------------------------------------------------------------
-// A wave holds four blocks of 256 elements, 16 lanes a block (a row of the lane crossbar): lane r of a row
-// has the elements j * 64 + r * 4 + 0..3, j = 0..3.  Each load of the wave then takes 256 contiguous bytes
-// of fp32 from each block, and a block's maximum is 4 row rotations, not 6 steps over the wave, for 16
-// elements a lane.
+// A wave holds a block of 256 elements, four a lane.
 
-constexpr int kGroup = 4 * CX_STATE_BLOCK;       // elements of a wave's four blocks
 constexpr float kTiny = 0x1p-100f;               // a block below is stored as zeros
 constexpr float kVUnit = 0x1.ep-96f;             // V lies here before its bits are cut: exponent field 31, fraction 7/8
 constexpr float kVBack = (float)(0x1p96 / 1.875);
 
-__device__ __forceinline__ unsigned row_max(unsigned x) {
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));  // rotate the row by 8
+// The wave's maximum, in every lane: four rotations within rows of 16 lanes, two broadcasts of a row's last
+// lane to the rows behind it, then lane 63 has seen all.
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));
     x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
     x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
     x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
-    return x;
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast:15
+    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // row_bcast:31
+    return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// The largest finite magnitude of a row's 64 x 4 values (floats of one sign order like their bits).
-__device__ __forceinline__ float block_max(const Vec4<float> (&x)[4]) {
+// The largest finite magnitude of the wave's values (floats of one sign are ordered like their bits).
+__device__ __forceinline__ float block_max(Vec4<float> x) {
     unsigned top = 0;
-    for (int j = 0; j < 4; ++j)
-        for (int k = 0; k < 4; ++k) {
-            const unsigned u = __float_as_uint(x[j][k]) & 0x7fffffffu;
-            top = max(top, u < 0x7f800000u ? u : 0u);
-        }
-    return __uint_as_float(row_max(top));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const unsigned u = __float_as_uint(x[k]) & 0x7fffffffu;
+        top = max(top, u < 0x7f800000u ? u : 0u);
+    }
+    return __uint_as_float(wave_max(top));
 }
 
 __device__ __forceinline__ Vec4<float> m_value(unsigned codes, float scale) {
@@ -126,12 +129,13 @@ __device__ __forceinline__ Vec4<float> m_value(unsigned codes, float scale) {
 }
 __device__ __forceinline__ Vec4<float> v_value(unsigned codes, float scale) {
     Vec4<float> x;
+#pragma unroll
     for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(((codes >> (8 * k)) & 255u) << 20);
     return x * kVBack * scale;
 }
 __device__ __forceinline__ unsigned m_codes(Vec4<float> m, float inverse) {
     m = m * inverse;
-    int u = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], 0, false);
+    const int u = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], 0, false);
     return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], u, true);
 }
 // The value's own exponent and upper fraction bits, after a scaling that leaves 5 bits of exponent: small
@@ -139,120 +143,101 @@ __device__ __forceinline__ unsigned m_codes(Vec4<float> m, float inverse) {
 __device__ __forceinline__ unsigned v_codes(Vec4<float> v, float inverse) {
     const Vec4<float> y = v * inverse * kVUnit;
     unsigned u = 0;
+#pragma unroll
     for (int k = 0; k < 4; ++k) {
-        unsigned code = min((__float_as_uint(y[k]) + 0x80000u) >> 20, 255u);
-        code = max(code, min(__float_as_uint(v[k]), 1u));  // above 0: never 0
-        u |= code << (8 * k);
+        const unsigned code = ((__float_as_uint(y[k]) + 0x80000u) >> 20) & 255u;   // (no finite value exceeds 255)
+        u |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * k);                 // above 0: never 0
     }
     return u;
 }
 
-// Rounds the moments of a row's block and stores codes and scales; lane `r` of the row, n elements of the
-// block there (at least one), `block` and the codes' base within the piece.
+// Rounds the moments of the wave's block and stores them: this lane's four codes of each (k of them exist) and
+// the block's scales.
 template <bool FULL>
-__device__ __forceinline__ void store_states(const Vec4<float> (&m)[4], const Vec4<float> (&v)[4], unsigned char* pm,
-                                             unsigned char* pv, float* sm, float* sv, int r, int n) {
+__device__ __forceinline__ void store_states(Vec4<float> m, Vec4<float> v, unsigned char* pm, unsigned char* pv, float* sm,
+                                             float* sv, int k) {
     const float mt = block_max(m), vt = block_max(v);
     const bool m_kept = mt >= kTiny, v_kept = vt >= kTiny;
-    const float m_inverse = m_kept ? 448.0f / mt : 0.0f, v_inverse = v_kept ? 1.0f / vt : 0.0f;
-    if (!FULL && n <= 0) return;
-    if (r == 0) {
-        *sm = m_kept ? mt * (float)(1.0 / 448.0) : 0.0f;
-        *sv = v_kept ? vt : 0.0f;
+    const unsigned mc = m_codes(m, m_kept ? 448.0f / mt : 0.0f);
+    const unsigned vc = v_kept ? v_codes(v, 1.0f / vt) : 0u;
+    store_up_to4<FULL>(pm, __builtin_bit_cast(Vec4<unsigned char>, mc), k);
+    store_up_to4<FULL>(pv, __builtin_bit_cast(Vec4<unsigned char>, vc), k);
+    if ((threadIdx.x & 63) == 0) {
+        *global(sm) = m_kept ? mt * (float)(1.0 / 448.0) : 0.0f;
+        *global(sv) = v_kept ? vt : 0.0f;
     }
-    for (int j = 0; j < 4; ++j) {
-        const int i = j * 64 + r * 4, k = FULL ? 4 : n - i;
-        const unsigned mc = m_codes(m[j], m_inverse), vc = v_kept ? v_codes(v[j], v_inverse) : 0u;
-        store_up_to4(pm + i, __builtin_bit_cast(Vec4<unsigned char>, mc), k);
-        store_up_to4(pv + i, __builtin_bit_cast(Vec4<unsigned char>, vc), k);
-    }
-}
-
-template <typename P, typename G, bool MASTER, bool FULL>
-__device__ __forceinline__ void adamw8_group(const Chunk& c, const G* g, int at, int r, int n, int block,
-                                             const AdamwArgs& a, const AdamwRates& rates, float f) {
-    P* p = static_cast<P*>(c.param) + at;
-    unsigned char *pm = static_cast<unsigned char*>(c.m) + at, *pv = static_cast<unsigned char*>(c.v) + at;
-    g += at;
-    const bool there = FULL || n > 0;
-    const float sm = there ? c.m_scale[block] : 0.0f, sv = there ? c.v_scale[block] : 0.0f;
-    Vec4<float> m[4], v[4];
-    for (int j = 0; j < 4; ++j) {
-        const int i = j * 64 + r * 4, k = FULL ? 4 : n - i;
-        const Vec4<float> x = to_float<G>(load_up_to4(g + i, k)) * f;
-        Vec4<float> w;
-        if constexpr (MASTER) w = load_up_to4(c.master + at + i, k);
-        else w = to_float<P>(load_up_to4(p + i, k));
-        m[j] = m_value(__builtin_bit_cast(unsigned, load_up_to4(pm + i, k)), sm);
-        v[j] = v_value(__builtin_bit_cast(unsigned, load_up_to4(pv + i, k)), sv);
-        moments(x, a, m[j], v[j]);
-        w = weights(w, m[j], v[j], a, rates);
-        if constexpr (MASTER) store_up_to4(c.master + at + i, w, k);
-        store_up_to4(p + i, from_float<P>(w), k);
-    }
-    store_states<FULL>(m, v, pm, pv, c.m_scale + block, c.v_scale + block, r, n);
 }
 
 template <typename P, typename G, bool MASTER>
-__global__ __launch_bounds__(kBlock) void adamw8_kernel(const Chunk* __restrict__ chunks, int first, GradArgs ga,
-                                                        AdamwArgs a) {
-    const Chunk c = chunks[first + blockIdx.x];
+__global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
+    const Piece c = piece_of<kFine>(ps);
     const G* g = grad_of<G>(c, ga);
     if (!g || (a.skip && *a.skip)) return;
-    const AdamwRates rates = a.device_rates ? *a.device_rates : a.rates;
+    const AdamwRates r = a.device_rates ? *a.device_rates : a.rates;
     const float f = factor_of(c, a.coefs, a.per_tensor, a.scale);
-    const int row = (threadIdx.x & 63) >> 4, r = threadIdx.x & 15;
-    for (int q = (threadIdx.x >> 6) * kGroup; q < c.n; q += kBlock / 64 * kGroup) {
-        const int at = q + row * CX_STATE_BLOCK, block = at / CX_STATE_BLOCK;
-        if (q + kGroup <= c.n) adamw8_group<P, G, MASTER, true>(c, g, at, r, CX_STATE_BLOCK, block, a, rates, f);
-        else adamw8_group<P, G, MASTER, false>(c, g, at, r, c.n - at, block, a, rates, f);
-    }
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave * CX_STATE_BLOCK >= c.n) return;
+    P* p = static_cast<P*>(c.t.param) + c.at;
+    unsigned char *pm = static_cast<unsigned char*>(c.t.m) + c.at, *pv = static_cast<unsigned char*>(c.t.v) + c.at;
+    float* pw = c.t.master + c.at;
+    const long long block = c.at / CX_STATE_BLOCK + wave;
+    float *sm = c.t.m_scale + block, *sv = c.t.v_scale + block;
+    const int i = threadIdx.x * 4, k = c.n - i;
+    by_length(c, [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const Vec4<G> gx = load_up_to4<FULL>(g + i, k);
+        const unsigned mc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pm + i, k));
+        const unsigned vc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pv + i, k));
+        Vec4<float> w;
+        if constexpr (MASTER) w = load_up_to4<FULL>(pw + i, k);
+        else w = to_float<P>(load_up_to4<FULL>(p + i, k));
+        Vec4<float> m = m_value(mc, *global(sm)), v = v_value(vc, *global(sv));
+        moments(to_float<G>(gx) * f, a, m, v);
+        w = weights(w, m, v, a, r);
+        if constexpr (MASTER) store_up_to4<FULL>(pw + i, w, k);
+        store_up_to4<FULL>(p + i, from_float<P>(w), k);
+        store_states<FULL>(m, v, pm + i, pv + i, sm, sv, k);
+    });
 }
 
 template <typename E>
-__global__ __launch_bounds__(kBlock) void states_kernel(const Chunk* __restrict__ chunks, E* __restrict__ m_out,
-                                                        E* __restrict__ v_out) {
-    const Chunk c = chunks[blockIdx.x];
-    const unsigned char *pm = static_cast<const unsigned char*>(c.m), *pv = static_cast<const unsigned char*>(c.v);
-    for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4) {
-        const int k = c.n - i, block = i / CX_STATE_BLOCK;
-        const Vec4<float> m = m_value(__builtin_bit_cast(unsigned, load_up_to4(pm + i, k)), c.m_scale[block]);
-        const Vec4<float> v = v_value(__builtin_bit_cast(unsigned, load_up_to4(pv + i, k)), c.v_scale[block]);
-        store_up_to4(m_out + c.flat + i, from_float<E>(m), k);
-        store_up_to4(v_out + c.flat + i, from_float<E>(v), k);
-    }
+__global__ __launch_bounds__(kBlock) void states_kernel(Pieces ps, E* __restrict__ m_out, E* __restrict__ v_out) {
+    const Piece c = piece_of<kFine>(ps);
+    const unsigned char *pm = static_cast<const unsigned char*>(c.t.m) + c.at, *pv = static_cast<const unsigned char*>(c.t.v) + c.at;
+    const int i = threadIdx.x * 4, k = c.n - i;
+    if (k <= 0) return;
+    const long long block = (c.at + i) / CX_STATE_BLOCK, to = c.t.flat + c.at + i;
+    by_length(c, [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const unsigned mc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pm + i, k));
+        const unsigned vc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pv + i, k));
+        store_up_to4<FULL>(m_out + to, from_float<E>(m_value(mc, global(c.t.m_scale)[block])), k);
+        store_up_to4<FULL>(v_out + to, from_float<E>(v_value(vc, global(c.t.v_scale)[block])), k);
+    });
 }
 
-__global__ __launch_bounds__(kBlock) void set_states_kernel(const Chunk* __restrict__ chunks,
-                                                            const float* __restrict__ m_in,
+__global__ __launch_bounds__(kBlock) void set_states_kernel(Pieces ps, const float* __restrict__ m_in,
                                                             const float* __restrict__ v_in) {
-    const Chunk c = chunks[blockIdx.x];
-    const int row = (threadIdx.x & 63) >> 4, r = threadIdx.x & 15;
-    for (int q = (threadIdx.x >> 6) * kGroup; q < c.n; q += kBlock / 64 * kGroup) {
-        const int at = q + row * CX_STATE_BLOCK, n = c.n - at, block = at / CX_STATE_BLOCK;
-        Vec4<float> m[4], v[4];
-        for (int j = 0; j < 4; ++j) {
-            const int i = at + j * 64 + r * 4, k = c.n - i;
-            m[j] = load_up_to4(m_in + c.flat + i, k);
-            v[j] = load_up_to4(v_in + c.flat + i, k);
-        }
-        store_states<false>(m, v, static_cast<unsigned char*>(c.m) + at, static_cast<unsigned char*>(c.v) + at,
-                            c.m_scale + block, c.v_scale + block, r, n);
-    }
+    const Piece c = piece_of<kFine>(ps);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave * CX_STATE_BLOCK >= c.n) return;
+    const int i = threadIdx.x * 4, k = c.n - i;
+    const long long from = c.t.flat + c.at + i, block = c.at / CX_STATE_BLOCK + wave;
+    store_states<false>(load_up_to4(m_in + from, k), load_up_to4(v_in + from, k), static_cast<unsigned char*>(c.t.m) + c.at + i,
+                 static_cast<unsigned char*>(c.t.v) + c.at + i, c.t.m_scale + block, c.t.v_scale + block, k);
 }
 
 template <typename P, typename G, bool MASTER>
-void launch_step(hipStream_t s, int bits, int n, const Chunk* chunks, int first, const GradArgs& g, const AdamwArgs& a) {
-    if (bits == 32) adamw32_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(chunks, first, g, a);
-    else adamw8_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(chunks, first, g, a);
+void launch_step(hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
+    if (bits == 32) adamw32_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
+    else adamw8_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
 }
 
 template <typename P, bool MASTER>
-void launch_step_for(int grad_type, hipStream_t s, int bits, int n, const Chunk* chunks, int first, const GradArgs& g,
-                     const AdamwArgs& a) {
-    if (grad_type == CX_F32) launch_step<P, float, MASTER>(s, bits, n, chunks, first, g, a);
-    else if (grad_type == CX_BF16) launch_step<P, __bf16, MASTER>(s, bits, n, chunks, first, g, a);
-    else launch_step<P, _Float16, MASTER>(s, bits, n, chunks, first, g, a);
+void launch_step_for(int grad_type, hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
+    if (grad_type == CX_F32) launch_step<P, float, MASTER>(s, bits, n, ps, g, a);
+    else if (grad_type == CX_BF16) launch_step<P, __bf16, MASTER>(s, bits, n, ps, g, a);
+    else launch_step<P, _Float16, MASTER>(s, bits, n, ps, g, a);
 }
 
 }  // namespace
@@ -277,30 +262,33 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
     } else {
         a.rates = rates_of(u->lr, u->beta1, u->beta2, u->weight_decay, (double)u->step);
     }
-    return for_grads(t, g, [&](int first, int n, const GradArgs& ga) -> int {
+    return for_grads(t, g, kFine, [&](const Pieces& ps, int n, const GradArgs& ga) -> int {
         const int bits = t->state_bits;
-        if (t->param_type == CX_F32) launch_step_for<float, false>(g->type, h->stream, bits, n, t->d_chunks, first, ga, a);
-        else if (t->param_type == CX_BF16 && t->masters) launch_step_for<__bf16, true>(g->type, h->stream, bits, n, t->d_chunks, first, ga, a);
-        else if (t->param_type == CX_BF16) launch_step_for<__bf16, false>(g->type, h->stream, bits, n, t->d_chunks, first, ga, a);
-        else if (t->masters) launch_step_for<_Float16, true>(g->type, h->stream, bits, n, t->d_chunks, first, ga, a);
-        else launch_step_for<_Float16, false>(g->type, h->stream, bits, n, t->d_chunks, first, ga, a);
+        if (t->param_type == CX_F32) launch_step_for<float, false>(g->type, h->stream, bits, n, ps, ga, a);
+        else if (t->param_type == CX_BF16 && t->masters) launch_step_for<__bf16, true>(g->type, h->stream, bits, n, ps, ga, a);
+        else if (t->param_type == CX_BF16) launch_step_for<__bf16, false>(g->type, h->stream, bits, n, ps, ga, a);
+        else if (t->masters) launch_step_for<_Float16, true>(g->type, h->stream, bits, n, ps, ga, a);
+        else launch_step_for<_Float16, false>(g->type, h->stream, bits, n, ps, ga, a);
         CX_HIP(hipGetLastError());
         return CX_OK;
     });
 }
 
 int launch_adamw_states(cx_handle h, cx_tensors t, int dt, void* d_m, void* d_v) {
-    if (t->chunks == 0) return CX_OK;
-    if (dt == CX_F32) states_kernel<<<t->chunks, kBlock, 0, h->stream>>>(t->d_chunks, static_cast<float*>(d_m), static_cast<float*>(d_v));
-    else if (dt == CX_BF16) states_kernel<<<t->chunks, kBlock, 0, h->stream>>>(t->d_chunks, static_cast<__bf16*>(d_m), static_cast<__bf16*>(d_v));
-    else states_kernel<<<t->chunks, kBlock, 0, h->stream>>>(t->d_chunks, static_cast<_Float16*>(d_m), static_cast<_Float16*>(d_v));
+    const int n = t->cut[kFine].pieces;
+    if (n == 0) return CX_OK;
+    const Pieces ps = t->pieces(kFine);
+    if (dt == CX_F32) states_kernel<<<n, kBlock, 0, h->stream>>>(ps, static_cast<float*>(d_m), static_cast<float*>(d_v));
+    else if (dt == CX_BF16) states_kernel<<<n, kBlock, 0, h->stream>>>(ps, static_cast<__bf16*>(d_m), static_cast<__bf16*>(d_v));
+    else states_kernel<<<n, kBlock, 0, h->stream>>>(ps, static_cast<_Float16*>(d_m), static_cast<_Float16*>(d_v));
     CX_HIP(hipGetLastError());
     return CX_OK;
 }
 
 int launch_adamw_set_states(cx_handle h, cx_tensors t, const float* d_m, const float* d_v) {
-    if (t->chunks == 0) return CX_OK;
-    set_states_kernel<<<t->chunks, kBlock, 0, h->stream>>>(t->d_chunks, d_m, d_v);
+    const int n = t->cut[kFine].pieces;
+    if (n == 0) return CX_OK;
+    set_states_kernel<<<n, kBlock, 0, h->stream>>>(t->pieces(kFine), d_m, d_v);
     CX_HIP(hipGetLastError());
     return CX_OK;
 }

@@ -32,19 +32,18 @@ template <int BLOCK> __device__ __forceinline__ double block_sum(double x) {
 
 // partial[piece] = sum of g^2.  64 bits: the squares of finite floats do not overflow there.
 template <typename G>
-__global__ __launch_bounds__(kBlock) void squares_kernel(const Chunk* __restrict__ chunks, int first, GradArgs ga,
-                                                         double* __restrict__ partial) {
-    const Chunk c = chunks[first + blockIdx.x];
+__global__ __launch_bounds__(kBlock) void squares_kernel(Pieces ps, GradArgs ga, double* __restrict__ partial) {
+    const Piece c = piece_of<kCoarse>(ps);
     const G* g = grad_of<G>(c, ga);
     double s = 0.0;
     if (g) {
         for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4) {
-            const Vec4<float> x = to_float<G>(load_up_to4(g + i, c.n - i));
+            const Vec4<float> x = to_float<G>(load_up_to4<false, true>(g + i, c.n - i));
             for (int k = 0; k < 4; ++k) s += (double)x[k] * (double)x[k];
         }
     }
     s = block_sum<kBlock>(s);
-    if (threadIdx.x == 0) partial[first + blockIdx.x] = s;
+    if (threadIdx.x == 0) partial[ps.first + dealt(blockIdx.x, gridDim.x)] = s;
 }
 
 __device__ __forceinline__ float clip_coef(double norm, double max_norm) {
@@ -53,11 +52,11 @@ __device__ __forceinline__ float clip_coef(double norm, double max_norm) {
 
 // Block t < count: tensor t's norm; block `count`: that of all, from all pieces' sums in a fixed order.
 __global__ __launch_bounds__(kBlock) void norms_kernel(const double* __restrict__ partial,
-                                                       const int* __restrict__ first_chunk, int count, double scale,
+                                                       const int* __restrict__ first_piece, int count, double scale,
                                                        double max_norm, int each, float* __restrict__ norms,
                                                        float* __restrict__ coefs, int* __restrict__ nonfinite) {
     const int t = blockIdx.x;
-    const int from = t < count ? first_chunk[t] : 0, to = first_chunk[t < count ? t + 1 : count];
+    const int from = t < count ? first_piece[t] : 0, to = first_piece[t < count ? t + 1 : count];
     double s = 0.0;
     for (int i = from + threadIdx.x; i < to; i += kBlock) s += partial[i];
     s = block_sum<kBlock>(s);
@@ -70,12 +69,11 @@ __global__ __launch_bounds__(kBlock) void norms_kernel(const double* __restrict_
 }
 
 template <typename G>
-__global__ __launch_bounds__(kBlock) void pack_kernel(const Chunk* __restrict__ chunks, int first, GradArgs ga,
-                                                      const float* __restrict__ coefs, int per_tensor, float scale,
+__global__ __launch_bounds__(kBlock) void pack_kernel(Pieces ps, GradArgs ga, const float* __restrict__ coefs, int per_tensor, float scale,
                                                       const int* __restrict__ skip, float* out) {
-    const Chunk c = chunks[first + blockIdx.x];
+    const Piece c = piece_of<kFine>(ps);
     const G* g = grad_of<G>(c, ga);
-    float* to = out + c.flat;
+    float* to = out + c.t.flat + c.at;
     if (!g || (skip && *skip)) {
         for (int i = threadIdx.x * 4; i < c.n; i += kBlock * 4) store_up_to4(to + i, Vec4<float>{}, c.n - i);
         return;
@@ -85,12 +83,16 @@ __global__ __launch_bounds__(kBlock) void pack_kernel(const Chunk* __restrict__ 
         store_up_to4(to + i, to_float<G>(load_up_to4(g + i, c.n - i)) * f, c.n - i);
 }
 
-// Elements per piece: a multiple of 1024, so that a piece of a tensor begins a block of 8-bit states.
-int chunk_elements(long long total) {
-    long long c = 1024;
-    while (c < 16384 && c * 2048 < total) c *= 2;
+// Elements of a coarse piece: at most some thousand partial sums.
+int coarse_step(long long total) {
+    long long c = 4096;
+    while (c < 65536 && c * 4096 < total) c *= 2;
     return (int)c;
 }
+
+// A launch has fewer than 2^32 threads, 256 for each piece of 1024 elements.
+constexpr long long kMostElements = 1ll << 33;
+constexpr int kMostTensors = 1 << 20;
 
 struct Span {
     uintptr_t from, to;
@@ -115,13 +117,13 @@ bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 
 int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale, double max_norm, int each,
                       float* d_norms, float* d_coefs, int* d_nonfinite) {
-    int rc = for_grads(t, g, [&](int first, int n, const GradArgs& a) -> int {
-        CX_NUM_DISPATCH(g->type, (squares_kernel<G><<<n, kBlock, 0, h->stream>>>(t->d_chunks, first, a, t->d_partial)));
+    int rc = for_grads(t, g, kCoarse, [&](const Pieces& ps, int n, const GradArgs& a) -> int {
+        CX_NUM_DISPATCH(g->type, (squares_kernel<G><<<n, kBlock, 0, h->stream>>>(ps, a, t->d_partial)));
         CX_HIP(hipGetLastError());
         return CX_OK;
     });
     if (rc != CX_OK) return rc;
-    norms_kernel<<<t->count + 1, kBlock, 0, h->stream>>>(t->d_partial, t->d_first_chunk, t->count, std::fabs(scale),
+    norms_kernel<<<t->count + 1, kBlock, 0, h->stream>>>(t->d_partial, t->cut[kCoarse].d_first, t->count, std::fabs(scale),
                                                          max_norm, each, d_norms, d_coefs, d_nonfinite);
     CX_HIP(hipGetLastError());
     return CX_OK;
@@ -129,8 +131,8 @@ int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale
 
 int launch_pack(cx_handle h, cx_tensors t, const cx_grads* g, const float* d_coefs, int n_coefs, float scale,
                 const int* d_skip, float* out) {
-    return for_grads(t, g, [&](int first, int n, const GradArgs& a) -> int {
-        CX_NUM_DISPATCH(g->type, (pack_kernel<G><<<n, kBlock, 0, h->stream>>>(t->d_chunks, first, a, d_coefs,
+    return for_grads(t, g, kFine, [&](const Pieces& ps, int n, const GradArgs& a) -> int {
+        CX_NUM_DISPATCH(g->type, (pack_kernel<G><<<n, kBlock, 0, h->stream>>>(ps, a, d_coefs,
                                                                               n_coefs != 1, scale, d_skip, out)));
         CX_HIP(hipGetLastError());
         return CX_OK;
@@ -177,11 +179,12 @@ int check_coefs(cx_tensors t, const float* d_coefs, int n_coefs, const char* who
 static int create_tensors(cx_tensors* out, cx_handle h, int count, const long long* sizes, const cx_adamw_state* state) {
     if (!out) return fail(CX_ERR_INVALID, "cx_tensors_create: null output");
     *out = nullptr;
-    if (!h || count < 0 || (count > 0 && !sizes)) return fail(CX_ERR_INVALID, "cx_tensors_create: bad arguments");
+    if (!h || count < 0 || count > kMostTensors || (count > 0 && !sizes)) return fail(CX_ERR_INVALID, "cx_tensors_create: bad arguments");
     long long total = 0;
     for (int k = 0; k < count; ++k) {
-        if (sizes[k] < 0 || sizes[k] > (1ll << 40) || (total += sizes[k]) > (1ll << 40))
-            return fail(CX_ERR_INVALID, "cx_tensors_create: tensor %d has a size of %lld", k, sizes[k]);
+        if (sizes[k] < 0) return fail(CX_ERR_INVALID, "cx_tensors_create: tensor %d has a size of %lld", k, sizes[k]);
+        if (sizes[k] > kMostElements || (total += sizes[k]) > kMostElements)
+            return fail(CX_ERR_INVALID, "cx_tensors_create: more than %lld elements: make more sets", kMostElements);
     }
     if (state) {
         if (!number_type(state->param_type))
@@ -224,8 +227,8 @@ static int create_tensors(cx_tensors* out, cx_handle h, int count, const long lo
 
     DeviceScope on(h->device);
     CX_HIP(on.error);
-    std::unique_ptr<cx_tensors_s, int (*)(cx_tensors)> owner(new cx_tensors_s(), cx_tensors_destroy);
-    cx_tensors t = owner.get();
+    std::unique_ptr<cx_tensors_s, int (*)(cx_tensors)> made(new cx_tensors_s(), cx_tensors_destroy);
+    cx_tensors t = made.get();
     t->device = h->device;
     t->count = count;
     t->total = total;
@@ -235,49 +238,56 @@ static int create_tensors(cx_tensors* out, cx_handle h, int count, const long lo
         t->state_bits = state->state_bits;
         t->masters = state->masters != nullptr;
     }
-    const int step = chunk_elements(total);
-    std::vector<Chunk> chunks;
+    t->cut[kFine].step = kFineStep;
+    t->cut[kCoarse].step = coarse_step(total);
+    std::vector<Tensor> tensors(count);
+    std::vector<int> owner[2];
     long long flat = 0;
     for (int k = 0; k < count; ++k) {
+        Tensor& x = tensors[k];
+        x = Tensor{};
+        x.n = sizes[k];
+        x.flat = flat;
+        if (state && sizes[k] > 0) {
+            x.param = state->params[k];
+            x.master = state->masters ? state->masters[k] : nullptr;
+            x.m = state->exp_avg[k];
+            x.v = state->exp_avg_sq[k];
+            if (state->state_bits == 8) {
+                x.m_scale = state->exp_avg_scales[k];
+                x.v_scale = state->exp_avg_sq_scales[k];
+            }
+        }
+        for (int w : {kFine, kCoarse}) {
+            (w == kFine ? x.first_fine : x.first_coarse) = (int)owner[w].size();
+            t->cut[w].first.push_back((int)owner[w].size());
+            owner[w].insert(owner[w].end(), (size_t)((sizes[k] + t->cut[w].step - 1) / t->cut[w].step), k);
+        }
         t->sizes.push_back(sizes[k]);
         t->flat.push_back(flat);
-        t->first_chunk.push_back((int)chunks.size());
-        for (long long at = 0; at < sizes[k]; at += step) {
-            Chunk c = {};
-            c.at = at;
-            c.flat = flat + at;
-            c.tensor = k;
-            c.n = (int)std::min<long long>(step, sizes[k] - at);
-            if (state) {
-                const long long pb = element_bytes(state->param_type), sb = state->state_bits / 8;
-                c.param = static_cast<char*>(state->params[k]) + at * pb;
-                c.master = state->masters ? state->masters[k] + at : nullptr;
-                c.m = static_cast<char*>(state->exp_avg[k]) + at * sb;
-                c.v = static_cast<char*>(state->exp_avg_sq[k]) + at * sb;
-                if (state->state_bits == 8) {
-                    c.m_scale = state->exp_avg_scales[k] + at / CX_STATE_BLOCK;
-                    c.v_scale = state->exp_avg_sq_scales[k] + at / CX_STATE_BLOCK;
-                }
-            }
-            chunks.push_back(c);
-        }
         flat += sizes[k];
     }
-    t->first_chunk.push_back((int)chunks.size());
-    t->chunks = (int)chunks.size();
-    const size_t nc = chunks.empty() ? 1 : chunks.size();
-    hipError_t e = hipMalloc(reinterpret_cast<void**>(&t->d_chunks), nc * sizeof(Chunk));
-    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_first_chunk), (count + 1) * sizeof(int));
-    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_partial), nc * sizeof(double));
+    hipError_t e = hipSuccess;
+    auto upload = [&](auto** to, const auto& from) {
+        if (e != hipSuccess) return;
+        const size_t bytes = from.size() * sizeof(from[0]);
+        e = hipMalloc(reinterpret_cast<void**>(to), bytes ? bytes : 1);
+        if (e == hipSuccess && bytes) e = hipMemcpyAsync(*to, from.data(), bytes, hipMemcpyHostToDevice, h->stream);
+    };
+    upload(&t->d_tensors, tensors);
+    for (int w : {kFine, kCoarse}) {
+        auto& cut = t->cut[w];
+        cut.pieces = (int)owner[w].size();
+        cut.first.push_back(cut.pieces);
+        upload(&cut.d_owner, owner[w]);
+        upload(&cut.d_first, cut.first);
+    }
+    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_partial), (t->cut[kCoarse].pieces + 1) * sizeof(double));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_rates), 256);
-    if (e == hipSuccess && !chunks.empty())
-        e = hipMemcpyAsync(t->d_chunks, chunks.data(), chunks.size() * sizeof(Chunk), hipMemcpyHostToDevice, h->stream);
-    if (e == hipSuccess)
-        e = hipMemcpyAsync(t->d_first_chunk, t->first_chunk.data(), (count + 1) * sizeof(int), hipMemcpyHostToDevice,
-                           h->stream);
-    if (e == hipSuccess) e = hipStreamSynchronize(h->stream);
+    const hipError_t waited = hipStreamSynchronize(h->stream);  // the host tables go away
+    if (e == hipSuccess) e = waited;
     if (e != hipSuccess) return fail(CX_ERR_HIP, "cx_tensors_create: %s", hipGetErrorString(e));
-    *out = owner.release();
+    *out = made.release();
     return CX_OK;
 }
 
@@ -294,8 +304,11 @@ int cx_tensors_create(cx_tensors* out, cx_handle h, int count, const long long* 
 int cx_tensors_destroy(cx_tensors t) {
     if (!t) return CX_OK;
     DeviceScope on(t->device);
-    if (t->d_chunks) (void)hipFree(t->d_chunks);  // waits for the device
-    if (t->d_first_chunk) (void)hipFree(t->d_first_chunk);
+    for (auto& cut : t->cut) {  // freeing waits for the device
+        if (cut.d_owner) (void)hipFree(cut.d_owner);
+        if (cut.d_first) (void)hipFree(cut.d_first);
+    }
+    if (t->d_tensors) (void)hipFree(t->d_tensors);
     if (t->d_partial) (void)hipFree(t->d_partial);
     if (t->d_rates) (void)hipFree(t->d_rates);
     delete t;

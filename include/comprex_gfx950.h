@@ -334,7 +334,7 @@ typedef struct {
     float* const* exp_avg_sq_scales;
 } cx_adamw_state;
 
-/* `sizes`: host array of element counts (0 allowed).  state == NULL: for cx_grad_norms and cx_pack only.
+/* `sizes`: host array of element counts (0 allowed), up to 2^20 tensors and 2^33 elements.  state == NULL: for cx_grad_norms and cx_pack only.
  * Refuses (CX_ERR_INVALID) buffers of `state` that overlap.  Waits for the handle's stream. */
 int cx_tensors_create(cx_tensors* out, cx_handle h, int count, const long long* sizes, const cx_adamw_state* state);
 int cx_tensors_destroy(cx_tensors t);

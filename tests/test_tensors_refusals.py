@@ -109,6 +109,8 @@ def test_c_entry_point_checks_before_it_touches_a_device():
     assert create(1, longs(-4)) == bad
     assert create(1, longs(1 << 41)) == bad
     assert create(2, longs(1 << 40, 1 << 40)) == bad
+    assert create(2, longs(1 << 33, 1)) == bad
+    assert create((1 << 20) + 1, longs(1)) == bad
 
     def state(**kw):
         a = (C.c_float * 64)()
