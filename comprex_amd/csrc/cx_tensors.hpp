@@ -9,12 +9,13 @@
 
 namespace cx {
 
+enum { kFine = 0, kWide = 1, kCoarse = 2, kDivisions = 3 };
+
 // One tensor.  A kernel reads one entry with scalar loads.
 struct alignas(16) Tensor {
     long long n;          // elements
     long long flat;       // first element within the flat vector of all tensors
-    int first_fine;       // first piece in each of the two divisions below
-    int first_coarse;
+    int first[kDivisions];  // first piece in each of the divisions below
     void* param;
     float* master;        // nullptr: none
     void* m;              // float or codes
@@ -25,11 +26,10 @@ struct alignas(16) Tensor {
 
 // The tensors are cut into pieces, one workgroup's work each; a tensor's last piece may be shorter.  `owner`
 // says which tensor a piece belongs to (4 bytes a piece, and the tensors' table stays in the caches).
-// kFine: everything that reads and writes.  Pieces of one load per stream and lane: all workgroups in flight
+// kFine and kWide: what reads and writes, 4 or 8 elements a lane.  Pieces of one load per stream and lane: all workgroups in flight
 // then walk through each buffer as one narrow front.  fp32 step on 25.6 M elements: 122 us with 1024 elements
 // a piece, 128 with 2048, 141 with 4096, 151 with 16384 (loops over the piece), 159 with 65536.
 // kCoarse: the sums of squares, which want few partial sums.
-enum { kFine = 0, kCoarse = 1 };
 struct Pieces {
     const Tensor* tensors;
     const int* owner;
@@ -57,7 +57,7 @@ template <int WHICH> __device__ __forceinline__ Piece piece_of(const Pieces& ps)
     const int id = ps.first + dealt(blockIdx.x, gridDim.x);
     c.tensor = __builtin_amdgcn_readfirstlane(ps.owner[id]);
     c.t = ps.tensors[c.tensor];
-    c.at = (long long)(id - (WHICH == kFine ? c.t.first_fine : c.t.first_coarse)) * ps.step;
+    c.at = (long long)(id - c.t.first[WHICH]) * ps.step;
     c.n = (int)min((long long)ps.step, c.t.n - c.at);
     return c;
 }
@@ -77,51 +77,49 @@ template <> struct Num<CX_F32> { using type = float; };
 template <> struct Num<CX_BF16> { using type = __bf16; };
 template <> struct Num<CX_F16> { using type = _Float16; };
 
-template <typename E> using Vec4 = E __attribute__((ext_vector_type(4)));
+template <typename E, int N> using Vec = E __attribute__((ext_vector_type(N)));
 
-// Four elements at any address that is aligned to one: gfx950's vector loads and stores take it.  The
-// addresses come out of a table, so the compiler has to be told that they are global memory.  Past the caches
+// N elements at any address that is aligned to one: gfx950's vector loads and stores take it.  The addresses
+// come out of a table, so the compiler has to be told that they are global memory.  Past the caches
 // (nontemporal) unless `KEEP`: a step touches everything once (fp32 step, 64 Mi elements in pieces of 2048: 355 us,
 // plain loads and stores 358 us, 25.6 M elements 128 and 147 us).
-template <bool KEEP = false, typename E>
-__device__ __forceinline__ Vec4<E> load4(const E* p) {
-    typedef Vec4<E> V __attribute__((aligned(sizeof(E))));
+template <int N, bool KEEP = false, typename E>
+__device__ __forceinline__ Vec<E, N> load(const E* p) {
+    typedef Vec<E, N> V __attribute__((aligned(sizeof(E))));
     auto* g = (const __attribute__((address_space(1))) V*)p;
     if constexpr (KEEP) return *g;
     else return __builtin_nontemporal_load(g);
 }
-template <typename E>
-__device__ __forceinline__ void store4(E* p, Vec4<E> x) {
-    typedef Vec4<E> V __attribute__((aligned(sizeof(E))));
+template <int N, typename E>
+__device__ __forceinline__ void store(E* p, Vec<E, N> x) {
+    typedef Vec<E, N> V __attribute__((aligned(sizeof(E))));
     __builtin_nontemporal_store(x, (__attribute__((address_space(1))) V*)p);
 }
 template <typename E> __device__ __forceinline__ __attribute__((address_space(1))) E* global(E* p) {
     return (__attribute__((address_space(1))) E*)p;
 }
-// The first `k` of them, zeros for the rest.  FULL: all four, without asking.
-template <bool FULL = false, bool KEEP = false, typename E>
-__device__ __forceinline__ Vec4<E> load_up_to4(const E* p, int k) {
-    if (FULL || k >= 4) return load4<KEEP>(p);
-    const auto* g = global(p);
-    Vec4<E> x = {};
-    if (k > 0) x[0] = g[0];
-    if (k > 1) x[1] = g[1];
-    if (k > 2) x[2] = g[2];
+// The first `k` of them, zeros for the rest.  FULL: all of them, without asking.
+template <int N, bool FULL = false, bool KEEP = false, typename E>
+__device__ __forceinline__ Vec<E, N> load_some(const E* p, int k) {
+    if (FULL || k >= N) return load<N, KEEP>(p);
+    Vec<E, N> x = {};
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i)
+        if (k > i) x[i] = global(p)[i];
     return x;
 }
-template <bool FULL = false, typename E>
-__device__ __forceinline__ void store_up_to4(E* p, Vec4<E> x, int k) {
-    if (FULL || k >= 4) return store4(p, x);
-    auto* g = global(p);
-    if (k > 0) g[0] = x[0];
-    if (k > 1) g[1] = x[1];
-    if (k > 2) g[2] = x[2];
+template <int N, bool FULL = false, typename E>
+__device__ __forceinline__ void store_some(E* p, Vec<E, N> x, int k) {
+    if (FULL || k >= N) return store<N>(p, x);
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i)
+        if (k > i) global(p)[i] = x[i];
 }
-template <typename E> __device__ __forceinline__ Vec4<float> to_float(Vec4<E> x) {
-    return __builtin_convertvector(x, Vec4<float>);
+template <int N, typename E> __device__ __forceinline__ Vec<float, N> to_float(Vec<E, N> x) {
+    return __builtin_convertvector(x, Vec<float, N>);
 }
-template <typename E> __device__ __forceinline__ Vec4<E> from_float(Vec4<float> x) {
-    return __builtin_convertvector(x, Vec4<E>);  // to nearest, ties to even
+template <typename E, int N> __device__ __forceinline__ Vec<E, N> from_float(Vec<float, N> x) {
+    return __builtin_convertvector(x, Vec<E, N>);  // to nearest, ties to even
 }
 
 // The gradient of a piece, nullptr where its tensor has none.
@@ -131,11 +129,10 @@ template <typename G> __device__ __forceinline__ const G* grad_of(const Piece& c
     return p ? p + c.at : nullptr;
 }
 
-// Calls body with true_type for a whole fine piece (no lane asks how many elements it has) and false_type for
+// Calls body with true_type for a whole piece (no lane asks how many elements it has) and false_type for
 // a tensor's last one.
-constexpr int kFineStep = 1024;
-template <typename F> __device__ __forceinline__ void by_length(const Piece& c, F&& body) {
-    if (c.n == kFineStep) body(std::true_type{});
+template <int STEP, typename F> __device__ __forceinline__ void by_length(const Piece& c, F&& body) {
+    if (c.n == STEP) body(std::true_type{});
     else body(std::false_type{});
 }
 
@@ -174,7 +171,7 @@ struct cx_tensors_s {
         std::vector<int> first;             // count + 1
         int* d_owner = nullptr;
         int* d_first = nullptr;             // `first` on the device
-    } cut[2];                               // kFine, kCoarse
+    } cut[cx::kDivisions];
     bool adamw = false;
     int param_type = 0, state_bits = 0;
     bool masters = false;

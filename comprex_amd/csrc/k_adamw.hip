@@ -15,7 +15,7 @@ namespace cx {
 
 namespace {
 
-constexpr int kBlock = 256;   // 4 elements a lane: a piece of 1024
+constexpr int kBlock = 256;   // 4 or 8 elements a lane: a fine or a wide piece
 
 // What depends on the step's count.
 struct AdamwRates {
@@ -49,187 +49,265 @@ __global__ void rates_kernel(int* count, long long step, const float* d_lr, doub
     *rates = rates_of(d_lr ? (double)*d_lr : lr, beta1, beta2, weight_decay, (double)step);
 }
 
-// The moments of four elements; g already has its factor.
-__device__ __forceinline__ void moments(Vec4<float> g, const AdamwArgs& a, Vec4<float>& m, Vec4<float>& v) {
+// The moments; g already has its factor.
+template <int N>
+__device__ __forceinline__ void moments(Vec<float, N> g, const AdamwArgs& a, Vec<float, N>& m, Vec<float, N>& v) {
     m = m * a.beta1 + g * a.rest1;
     v = v * a.beta2 + g * g * a.rest2;
 }
 
-__device__ __forceinline__ Vec4<float> weights(Vec4<float> w, Vec4<float> m, Vec4<float> v, const AdamwArgs& a,
-                                               const AdamwRates& r) {
+template <int N>
+__device__ __forceinline__ Vec<float, N> weights(Vec<float, N> w, Vec<float, N> m, Vec<float, N> v, const AdamwArgs& a,
+                                                 const AdamwRates& r) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float below = __builtin_fmaf(__builtin_sqrtf(v[k]), r.v_unit, a.eps);
-        w[k] -= __builtin_fmaf(r.decay, w[k], r.step * (m[k] / below));
+    for (int k = 0; k < N; ++k) {
+        const float below = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[k]), r.v_unit, a.eps);
+        w[k] -= __builtin_fmaf(r.decay, w[k], r.step * (m[k] * __builtin_amdgcn_rcpf(below)));
     }
     return w;
 }
 
-// One piece a workgroup, four elements a lane: everything is asked for before anything is used.
-template <typename P, typename G, bool MASTER>
+// One piece a workgroup, N elements a lane: everything is asked for before anything is used.
+template <int N, typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kBlock) void adamw32_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
-    const Piece c = piece_of<kFine>(ps);
+    const Piece c = piece_of<N == 4 ? kFine : kWide>(ps);
     const G* g = grad_of<G>(c, ga);
     if (!g || (a.skip && *a.skip)) return;
     const AdamwRates r = a.device_rates ? *a.device_rates : a.rates;
     const float f = factor_of(c, a.coefs, a.per_tensor, a.scale);
     P* p = static_cast<P*>(c.t.param) + c.at;
     float *pm = static_cast<float*>(c.t.m) + c.at, *pv = static_cast<float*>(c.t.v) + c.at, *pw = c.t.master + c.at;
-    const int i = threadIdx.x * 4, k = c.n - i;
+    const int i = threadIdx.x * N, k = c.n - i;
     if (k <= 0) return;
-    by_length(c, [&](auto full) {
+    by_length<kBlock * N>(c, [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        const Vec4<G> gx = load_up_to4<FULL>(g + i, k);
-        Vec4<float> m = load_up_to4<FULL>(pm + i, k), v = load_up_to4<FULL>(pv + i, k);
-        Vec4<float> w;
-        if constexpr (MASTER) w = load_up_to4<FULL>(pw + i, k);
-        else w = to_float<P>(load_up_to4<FULL>(p + i, k));
-        moments(to_float<G>(gx) * f, a, m, v);
-        w = weights(w, m, v, a, r);
-        store_up_to4<FULL>(pm + i, m, k);
-        store_up_to4<FULL>(pv + i, v, k);
-        if constexpr (MASTER) store_up_to4<FULL>(pw + i, w, k);
-        store_up_to4<FULL>(p + i, from_float<P>(w), k);
+        const Vec<G, N> gx = load_some<N, FULL>(g + i, k);
+        Vec<float, N> m = load_some<N, FULL>(pm + i, k), v = load_some<N, FULL>(pv + i, k), w;
+        if constexpr (MASTER) w = load_some<N, FULL>(pw + i, k);
+        else w = to_float<N>(load_some<N, FULL>(p + i, k));
+        moments<N>(to_float<N>(gx) * f, a, m, v);
+        w = weights<N>(w, m, v, a, r);
+        store_some<N, FULL>(pm + i, m, k);
+        store_some<N, FULL>(pv + i, v, k);
+        if constexpr (MASTER) store_some<N, FULL>(pw + i, w, k);
+        store_some<N, FULL>(p + i, from_float<P, N>(w), k);
     });
 }
 
 // ---- 8-bit moments ---------------------------------------------------------------------------
-// A wave holds a block of 256 elements, four a lane.
+// Half a wave holds a block of 256 elements, eight a lane.  Four a lane, a block per wave, took 190 us where this takes
+// 158 (100 M bf16 weights): twice the waves, each with its way to its piece, its maxima and its quotients.
+// A lane's eight are neighbours where weights and gradients have 16 bits (16 bytes a load); where one of them has
+// 32 they are two fours, 128 elements apart, so that every load of the wave still covers whole stretches of 512
+// bytes (fp32, 25.6 M weights: neighbours 84 us, fours 68 us).
+template <bool SPLIT, bool FULL> struct Eight {
+    int at, other, n;    // first elements of the two fours within the piece; the piece's length
+    __device__ __forceinline__ explicit Eight(int length) : n(length) {
+        const int lane = threadIdx.x & 31;
+        at = (threadIdx.x >> 5) * CX_STATE_BLOCK + (SPLIT ? lane * 4 : lane * 8);
+        other = at + (SPLIT ? 128 : 4);
+    }
+    template <typename E> __device__ __forceinline__ Vec<E, 8> load(const E* p) const {
+        if constexpr (SPLIT) {
+            const Vec<E, 4> a = load_some<4, FULL>(p + at, n - at), b = load_some<4, FULL>(p + other, n - other);
+            return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return load_some<8, FULL>(p + at, n - at);
+        }
+    }
+    template <typename E> __device__ __forceinline__ void store(E* p, Vec<E, 8> x) const {
+        if constexpr (SPLIT) {
+            store_some<4, FULL>(p + at, __builtin_shufflevector(x, x, 0, 1, 2, 3), n - at);
+            store_some<4, FULL>(p + other, __builtin_shufflevector(x, x, 4, 5, 6, 7), n - other);
+        } else {
+            store_some<8, FULL>(p + at, x, n - at);
+        }
+    }
+};
 
 constexpr float kTiny = 0x1p-100f;               // a block below is stored as zeros
 constexpr float kVUnit = 0x1.ep-96f;             // V lies here before its bits are cut: exponent field 31, fraction 7/8
 constexpr float kVBack = (float)(0x1p96 / 1.875);
 
-// The wave's maximum, in every lane: four rotations within rows of 16 lanes, two broadcasts of a row's last
-// lane to the rows behind it, then lane 63 has seen all.
-__device__ __forceinline__ unsigned wave_max(unsigned x) {
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false));  // row_bcast:15
-    x = max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false));  // row_bcast:31
-    return (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+struct Codes { unsigned x[2]; };                 // eight of them
+using Bytes = Vec<unsigned char, 8>;
+
+// Two maxima over each half of the wave, left in its last lane: four rotations within rows of 16 lanes, then
+// every other row takes the row before it along.
+__device__ __forceinline__ void half_max(unsigned& a, unsigned& b) {
+#define CX_STEP(ctrl, rows)                                                                   \
+    {                                                                                         \
+        const unsigned x = (unsigned)__builtin_amdgcn_update_dpp(0, (int)a, ctrl, rows, 0xf, false); \
+        const unsigned y = (unsigned)__builtin_amdgcn_update_dpp(0, (int)b, ctrl, rows, 0xf, false); \
+        a = max(a, x);                                                                        \
+        b = max(b, y);                                                                        \
+    }
+    CX_STEP(0x128, 0xf)  // row_ror:8
+    CX_STEP(0x124, 0xf)
+    CX_STEP(0x122, 0xf)
+    CX_STEP(0x121, 0xf)
+    CX_STEP(0x142, 0xa)  // row_bcast:15 into rows 1 and 3
+#undef CX_STEP
 }
 
-// The largest finite magnitude of the wave's values (floats of one sign are ordered like their bits).
-__device__ __forceinline__ float block_max(Vec4<float> x) {
+// The largest magnitude among a lane's values; NaN only where there is nothing else.
+__device__ __forceinline__ unsigned lane_max(Vec<float, 8> x) {
+    float t = __builtin_fabsf(x[0]);
+#pragma unroll
+    for (int k = 1; k < 8; ++k) t = __builtin_fmaxf(t, __builtin_fabsf(x[k]));
+    return __float_as_uint(t);
+}
+// ... among the finite ones
+__device__ __forceinline__ unsigned lane_max_finite(Vec<float, 8> x) {
     unsigned top = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
         const unsigned u = __float_as_uint(x[k]) & 0x7fffffffu;
         top = max(top, u < 0x7f800000u ? u : 0u);
     }
-    return __uint_as_float(wave_max(top));
+    return top;
 }
 
-__device__ __forceinline__ Vec4<float> m_value(unsigned codes, float scale) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-    return Vec4<float>{lo[0], lo[1], hi[0], hi[1]} * scale;
-}
-__device__ __forceinline__ Vec4<float> v_value(unsigned codes, float scale) {
-    Vec4<float> x;
+__device__ __forceinline__ Vec<float, 8> m_value(Codes c, float scale) {
+    Vec<float, 8> x;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(((codes >> (8 * k)) & 255u) << 20);
+    for (int j = 0; j < 2; ++j) {
+        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c.x[j], true);
+        x[4 * j] = lo[0];
+        x[4 * j + 1] = lo[1];
+        x[4 * j + 2] = hi[0];
+        x[4 * j + 3] = hi[1];
+    }
+    return x * scale;
+}
+__device__ __forceinline__ Vec<float, 8> v_value(Codes c, float scale) {
+    Vec<float, 8> x;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(((c.x[k / 4] >> (8 * (k % 4))) & 255u) << 20);
     return x * kVBack * scale;
 }
-__device__ __forceinline__ unsigned m_codes(Vec4<float> m, float inverse) {
+__device__ __forceinline__ Codes m_codes(Vec<float, 8> m, float inverse) {
     m = m * inverse;
-    const int u = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], 0, false);
-    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], u, true);
+    Codes c;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int u = __builtin_amdgcn_cvt_pk_fp8_f32(m[4 * j], m[4 * j + 1], 0, false);
+        c.x[j] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(m[4 * j + 2], m[4 * j + 3], u, true);
+    }
+    return c;
 }
 // The value's own exponent and upper fraction bits, after a scaling that leaves 5 bits of exponent: small
 // values run into the format's subnormals as they do into those of fp32.  Rounded to nearest.
-__device__ __forceinline__ unsigned v_codes(Vec4<float> v, float inverse) {
-    const Vec4<float> y = v * inverse * kVUnit;
-    unsigned u = 0;
+__device__ __forceinline__ Codes v_codes(Vec<float, 8> v, float inverse) {
+    const Vec<float, 8> y = v * inverse * kVUnit;
+    Codes c = {};
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 8; ++k) {
         const unsigned code = ((__float_as_uint(y[k]) + 0x80000u) >> 20) & 255u;   // (no finite value exceeds 255)
-        u |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * k);                 // above 0: never 0
+        c.x[k / 4] |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * (k % 4));  // above 0: never 0
     }
-    return u;
+    return c;
 }
 
-// Rounds the moments of the wave's block and stores them: this lane's four codes of each (k of them exist) and
-// the block's scales.
-template <bool FULL>
-__device__ __forceinline__ void store_states(Vec4<float> m, Vec4<float> v, unsigned char* pm, unsigned char* pv, float* sm,
-                                             float* sv, int k) {
-    const float mt = block_max(m), vt = block_max(v);
-    const bool m_kept = mt >= kTiny, v_kept = vt >= kTiny;
-    const unsigned mc = m_codes(m, m_kept ? 448.0f / mt : 0.0f);
-    const unsigned vc = v_kept ? v_codes(v, 1.0f / vt) : 0u;
-    store_up_to4<FULL>(pm, __builtin_bit_cast(Vec4<unsigned char>, mc), k);
-    store_up_to4<FULL>(pv, __builtin_bit_cast(Vec4<unsigned char>, vc), k);
-    if ((threadIdx.x & 63) == 0) {
-        *global(sm) = m_kept ? mt * (float)(1.0 / 448.0) : 0.0f;
-        *global(sv) = v_kept ? vt : 0.0f;
+__device__ __forceinline__ unsigned lane_of(unsigned x, int lane) {
+    return (unsigned)__builtin_amdgcn_readlane((int)x, lane);
+}
+
+// Rounds the moments of the wave's two blocks and stores them: the codes and the blocks' scales, sm and sv being
+// those of the wave's first one; `blocks` of them exist.
+template <bool SPLIT, bool FULL>
+__device__ __forceinline__ void store_states(const Eight<SPLIT, FULL>& e, Vec<float, 8> m, Vec<float, 8> v, unsigned char* pm,
+                                             unsigned char* pv, float* sm, float* sv, int blocks) {
+    unsigned mt = lane_max(m), vt = lane_max(v);
+    half_max(mt, vt);
+    if (max(max(lane_of(mt, 31), lane_of(mt, 63)), max(lane_of(vt, 31), lane_of(vt, 63))) >= 0x7f800000u) {
+        // an infinity, or a lane that has only NaN: once more without them
+        mt = lane_max_finite(m);
+        vt = lane_max_finite(v);
+        half_max(mt, vt);
     }
+    // the four quotients at once, one in each row: m and v of the first block, m and v of the second
+    const int lane = threadIdx.x & 63;
+    const bool of_v = lane & 16, second = lane & 32;
+    const float top = __uint_as_float(second ? (of_v ? lane_of(vt, 63) : lane_of(mt, 63)) : (of_v ? lane_of(vt, 31) : lane_of(mt, 31)));
+    const bool kept = top >= kTiny;
+    const unsigned quotient = __float_as_uint(kept ? (of_v ? 1.0f : 448.0f) / top : 0.0f);
+    const float m_inverse = __uint_as_float(second ? lane_of(quotient, 32) : lane_of(quotient, 0));
+    const float v_inverse = __uint_as_float(second ? lane_of(quotient, 48) : lane_of(quotient, 16));
+    const Codes mc = m_codes(m, m_inverse), all = v_codes(v, v_inverse);
+    const bool v_kept = v_inverse > 0.0f;
+    const Codes vc = {v_kept ? all.x[0] : 0u, v_kept ? all.x[1] : 0u};
+    e.store(pm, __builtin_bit_cast(Bytes, mc));
+    e.store(pv, __builtin_bit_cast(Bytes, vc));
+    const int b = lane >> 5;
+    if ((lane & 15) == 0 && (FULL || b < blocks))
+        global(of_v ? sv : sm)[b] = kept ? (of_v ? top : top * (float)(1.0 / 448.0)) : 0.0f;
 }
 
 template <typename P, typename G, bool MASTER>
 __global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
-    const Piece c = piece_of<kFine>(ps);
+    const Piece c = piece_of<kWide>(ps);
     const G* g = grad_of<G>(c, ga);
     if (!g || (a.skip && *a.skip)) return;
     const AdamwRates r = a.device_rates ? *a.device_rates : a.rates;
     const float f = factor_of(c, a.coefs, a.per_tensor, a.scale);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (wave * CX_STATE_BLOCK >= c.n) return;
+    const int blocks = (c.n - wave * 512 + CX_STATE_BLOCK - 1) / CX_STATE_BLOCK;  // of this wave's two
+    if (blocks <= 0) return;
     P* p = static_cast<P*>(c.t.param) + c.at;
     unsigned char *pm = static_cast<unsigned char*>(c.t.m) + c.at, *pv = static_cast<unsigned char*>(c.t.v) + c.at;
     float* pw = c.t.master + c.at;
-    const long long block = c.at / CX_STATE_BLOCK + wave;
+    const long long block = c.at / CX_STATE_BLOCK + wave * 2;
     float *sm = c.t.m_scale + block, *sv = c.t.v_scale + block;
-    const int i = threadIdx.x * 4, k = c.n - i;
-    by_length(c, [&](auto full) {
+    by_length<kBlock * 8>(c, [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        const Vec4<G> gx = load_up_to4<FULL>(g + i, k);
-        const unsigned mc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pm + i, k));
-        const unsigned vc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pv + i, k));
-        Vec4<float> w;
-        if constexpr (MASTER) w = load_up_to4<FULL>(pw + i, k);
-        else w = to_float<P>(load_up_to4<FULL>(p + i, k));
-        Vec4<float> m = m_value(mc, *global(sm)), v = v_value(vc, *global(sv));
-        moments(to_float<G>(gx) * f, a, m, v);
-        w = weights(w, m, v, a, r);
-        if constexpr (MASTER) store_up_to4<FULL>(pw + i, w, k);
-        store_up_to4<FULL>(p + i, from_float<P>(w), k);
-        store_states<FULL>(m, v, pm + i, pv + i, sm, sv, k);
+        constexpr bool SPLIT = MASTER || sizeof(P) == 4 || sizeof(G) == 4;
+        const Eight<SPLIT, FULL> e(c.n);
+        const Vec<G, 8> gx = e.load(g);
+        const Codes mc = __builtin_bit_cast(Codes, e.load(pm)), vc = __builtin_bit_cast(Codes, e.load(pv));
+        Vec<float, 8> w;
+        if constexpr (MASTER) w = e.load(pw);
+        else w = to_float<8>(e.load(p));
+        const int mine = FULL || blocks > 1 ? (threadIdx.x >> 5) & 1 : 0;
+        Vec<float, 8> m = m_value(mc, global(sm)[mine]), v = v_value(vc, global(sv)[mine]);
+        moments<8>(to_float<8>(gx) * f, a, m, v);
+        w = weights<8>(w, m, v, a, r);
+        if constexpr (MASTER) e.store(pw, w);
+        e.store(p, from_float<P, 8>(w));
+        store_states(e, m, v, pm, pv, sm, sv, blocks);
     });
 }
 
 template <typename E>
 __global__ __launch_bounds__(kBlock) void states_kernel(Pieces ps, E* __restrict__ m_out, E* __restrict__ v_out) {
-    const Piece c = piece_of<kFine>(ps);
+    const Piece c = piece_of<kWide>(ps);
+    const int in_piece = threadIdx.x >> 5;
+    if (in_piece * CX_STATE_BLOCK >= c.n) return;
     const unsigned char *pm = static_cast<const unsigned char*>(c.t.m) + c.at, *pv = static_cast<const unsigned char*>(c.t.v) + c.at;
-    const int i = threadIdx.x * 4, k = c.n - i;
-    if (k <= 0) return;
-    const long long block = (c.at + i) / CX_STATE_BLOCK, to = c.t.flat + c.at + i;
-    by_length(c, [&](auto full) {
-        constexpr bool FULL = decltype(full)::value;
-        const unsigned mc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pm + i, k));
-        const unsigned vc = __builtin_bit_cast(unsigned, load_up_to4<FULL>(pv + i, k));
-        store_up_to4<FULL>(m_out + to, from_float<E>(m_value(mc, global(c.t.m_scale)[block])), k);
-        store_up_to4<FULL>(v_out + to, from_float<E>(v_value(vc, global(c.t.v_scale)[block])), k);
+    const long long block = c.at / CX_STATE_BLOCK + in_piece, to = c.t.flat + c.at;
+    by_length<kBlock * 8>(c, [&](auto full) {
+        const Eight<sizeof(E) == 4, decltype(full)::value> e(c.n);
+        const Codes mc = __builtin_bit_cast(Codes, e.load(pm)), vc = __builtin_bit_cast(Codes, e.load(pv));
+        e.store(m_out + to, from_float<E, 8>(m_value(mc, global(c.t.m_scale)[block])));
+        e.store(v_out + to, from_float<E, 8>(v_value(vc, global(c.t.v_scale)[block])));
     });
 }
 
 __global__ __launch_bounds__(kBlock) void set_states_kernel(Pieces ps, const float* __restrict__ m_in,
                                                             const float* __restrict__ v_in) {
-    const Piece c = piece_of<kFine>(ps);
+    const Piece c = piece_of<kWide>(ps);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (wave * CX_STATE_BLOCK >= c.n) return;
-    const int i = threadIdx.x * 4, k = c.n - i;
-    const long long from = c.t.flat + c.at + i, block = c.at / CX_STATE_BLOCK + wave;
-    store_states<false>(load_up_to4(m_in + from, k), load_up_to4(v_in + from, k), static_cast<unsigned char*>(c.t.m) + c.at + i,
-                 static_cast<unsigned char*>(c.t.v) + c.at + i, c.t.m_scale + block, c.t.v_scale + block, k);
+    const int blocks = (c.n - wave * 512 + CX_STATE_BLOCK - 1) / CX_STATE_BLOCK;
+    if (blocks <= 0) return;
+    const long long from = c.t.flat + c.at, block = c.at / CX_STATE_BLOCK + wave * 2;
+    const Eight<true, false> e(c.n);
+    store_states(e, e.load(m_in + from), e.load(v_in + from), static_cast<unsigned char*>(c.t.m) + c.at,
+                 static_cast<unsigned char*>(c.t.v) + c.at, c.t.m_scale + block, c.t.v_scale + block, blocks);
 }
 
 template <typename P, typename G, bool MASTER>
 void launch_step(hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
-    if (bits == 32) adamw32_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
+    if (bits == 32) adamw32_kernel<4, P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
     else adamw8_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
 }
 
@@ -262,7 +340,7 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
     } else {
         a.rates = rates_of(u->lr, u->beta1, u->beta2, u->weight_decay, (double)u->step);
     }
-    return for_grads(t, g, kFine, [&](const Pieces& ps, int n, const GradArgs& ga) -> int {
+    return for_grads(t, g, t->state_bits == 32 ? kFine : kWide, [&](const Pieces& ps, int n, const GradArgs& ga) -> int {
         const int bits = t->state_bits;
         if (t->param_type == CX_F32) launch_step_for<float, false>(g->type, h->stream, bits, n, ps, ga, a);
         else if (t->param_type == CX_BF16 && t->masters) launch_step_for<__bf16, true>(g->type, h->stream, bits, n, ps, ga, a);
@@ -275,9 +353,9 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
 }
 
 int launch_adamw_states(cx_handle h, cx_tensors t, int dt, void* d_m, void* d_v) {
-    const int n = t->cut[kFine].pieces;
+    const int n = t->cut[kWide].pieces;
     if (n == 0) return CX_OK;
-    const Pieces ps = t->pieces(kFine);
+    const Pieces ps = t->pieces(kWide);
     if (dt == CX_F32) states_kernel<<<n, kBlock, 0, h->stream>>>(ps, static_cast<float*>(d_m), static_cast<float*>(d_v));
     else if (dt == CX_BF16) states_kernel<<<n, kBlock, 0, h->stream>>>(ps, static_cast<__bf16*>(d_m), static_cast<__bf16*>(d_v));
     else states_kernel<<<n, kBlock, 0, h->stream>>>(ps, static_cast<_Float16*>(d_m), static_cast<_Float16*>(d_v));
@@ -286,9 +364,9 @@ int launch_adamw_states(cx_handle h, cx_tensors t, int dt, void* d_m, void* d_v)
 }
 
 int launch_adamw_set_states(cx_handle h, cx_tensors t, const float* d_m, const float* d_v) {
-    const int n = t->cut[kFine].pieces;
+    const int n = t->cut[kWide].pieces;
     if (n == 0) return CX_OK;
-    set_states_kernel<<<n, kBlock, 0, h->stream>>>(t->pieces(kFine), d_m, d_v);
+    set_states_kernel<<<n, kBlock, 0, h->stream>>>(t->pieces(kWide), d_m, d_v);
     CX_HIP(hipGetLastError());
     return CX_OK;
 }

@@ -247,11 +247,12 @@ def check_step(P, before, g, factor, step, lr, b1, b2, eps, wd, tensors=None):
         ev = U * ((2 + 3 * small) * b2 * v + 10 * (1 - b2) * x * x + 1.01 * v1) + 2.0 ** -147
         unit = 1 / math.sqrt(1 - b2 ** step)
         below = np.sqrt(v1) * unit + eps
-        # sqrt of the range of v, its rounding, v_unit, the sum's rounding, eps
-        eb = (np.sqrt(v1 + ev) - np.sqrt(np.maximum(v1 - ev, 0))) * unit + 4.01 * U * below
+        # sqrt of the range of v, the square root itself (one unit in the last place: 2 u), v_unit, the sum's rounding, eps
+        eb = (np.sqrt(v1 + ev) - np.sqrt(np.maximum(v1 - ev, 0))) * unit + 5.01 * U * below
         rate = lr / (1 - b1 ** step)
         move = rate * m1 / below
-        em_move = rate * em / below + np.abs(move) * (eb / (below - eb) + 4.01 * U)
+        # the reciprocal (one unit in the last place: 2 u), its product with m, the rate, the product with it
+        em_move = rate * em / below + np.abs(move) * (eb / (below - eb) + 5.01 * U)
         w1 = w - lr * wd * w - move
         ew = em_move + U * (3 * np.abs(lr * wd * w) + 2 * np.abs(move) + 1.01 * np.abs(w1))
         got_w, got_m, got_v = P.now()[k]
