@@ -15,7 +15,8 @@ F32 = torch.float32
 def host_set(sizes, cls=TensorSet):
     """A set whose checks run on host tensors; it has no device part."""
     s = cls.__new__(cls)
-    s.sizes, s.total, s.device = sizes, sum(sizes), torch.device("cpu")
+    s.sizes, s.total = sizes, sum(sizes)
+    s._on(torch.device("cpu"))
     return s
 
 
@@ -28,21 +29,25 @@ def refused(code, f, *args, **kw):
 def test_gradients_are_checked():
     s = host_set([3, 0, 5])
     good = [torch.zeros(3), torch.zeros(0), torch.zeros(1, 5)]
-    assert s._grads(good).type == _lib.CX_F32
-    assert s._grads([None, None, torch.zeros(5, dtype=torch.bfloat16)]).type == _lib.CX_BF16
-    assert s._grads([None] * 3).type == _lib.CX_F32
-    assert s._grads(torch.zeros(8, dtype=torch.float16)).type == _lib.CX_F16
+    assert s.gradients(good).type == _lib.CX_F32
+    assert s.gradients([None, None, torch.zeros(5, dtype=torch.bfloat16)]).type == _lib.CX_BF16
+    assert s.gradients([None] * 3).type == _lib.CX_F32
+    assert s.gradients(torch.zeros(8, dtype=torch.float16)).type == _lib.CX_F16
     bad, size = _lib.CX_ERR_INVALID, _lib.CX_ERR_SIZE_MISMATCH
-    refused(size, s._grads, good[:2])
-    refused(size, s._grads, [torch.zeros(4), good[1], good[2]])
-    refused(size, s._grads, torch.zeros(7))
-    refused(size, s._grads, torch.zeros(2, 4))
-    refused(bad, s._grads, [torch.zeros(3, dtype=torch.bfloat16), None, torch.zeros(5)])   # two types
-    refused(bad, s._grads, [torch.zeros(3, dtype=torch.float64), None, None])
-    refused(bad, s._grads, torch.zeros(8, dtype=torch.int32))
-    refused(bad, s._grads, [torch.zeros(6)[::2], None, None])                             # strided
-    refused(bad, s._grads, [None, None, torch.zeros(5, device="meta")])
-    refused(bad, s._grads, torch.zeros(16)[::2])
+    ready = s.gradients(good)
+    assert s.gradients(ready) is ready
+    refused(bad, host_set([3, 0, 5]).gradients, ready)                                    # made for another set
+    refused(bad, host_set([8]).gradients, s.gradients(torch.zeros(8)))
+    refused(size, s.gradients, good[:2])
+    refused(size, s.gradients, [torch.zeros(4), good[1], good[2]])
+    refused(size, s.gradients, torch.zeros(7))
+    refused(size, s.gradients, torch.zeros(2, 4))
+    refused(bad, s.gradients, [torch.zeros(3, dtype=torch.bfloat16), None, torch.zeros(5)])   # two types
+    refused(bad, s.gradients, [torch.zeros(3, dtype=torch.float64), None, None])
+    refused(bad, s.gradients, torch.zeros(8, dtype=torch.int32))
+    refused(bad, s.gradients, [torch.zeros(6)[::2], None, None])                             # strided
+    refused(bad, s.gradients, [None, None, torch.zeros(5, device="meta")])
+    refused(bad, s.gradients, torch.zeros(16)[::2])
 
 
 def test_vectors_coefficients_and_single_values_are_checked():
