@@ -31,6 +31,7 @@ struct AdamwArgs {
     const float* coefs;
     int per_tensor;
     const int* skip;
+    float* moves;                                   // where the moves go, if not into the weights
 };
 
 __host__ __device__ inline AdamwRates rates_of(double lr, double beta1, double beta2, double weight_decay, double t) {
@@ -57,40 +58,76 @@ __device__ __forceinline__ void moments(Vec<float, N> g, const AdamwArgs& a, Vec
 }
 
 template <int N>
-__device__ __forceinline__ Vec<float, N> weights(Vec<float, N> w, Vec<float, N> m, Vec<float, N> v, const AdamwArgs& a,
-                                                 const AdamwRates& r) {
+__device__ __forceinline__ Vec<float, N> moves_of(Vec<float, N> m, Vec<float, N> v, const AdamwArgs& a, const AdamwRates& r) {
+    Vec<float, N> x;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         const float below = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[k]), r.v_unit, a.eps);
-        w[k] -= __builtin_fmaf(r.decay, w[k], r.step * (m[k] * __builtin_amdgcn_rcpf(below)));
+        x[k] = r.step * (m[k] * __builtin_amdgcn_rcpf(below));
     }
+    return x;
+}
+
+template <int N> __device__ __forceinline__ Vec<float, N> moved(Vec<float, N> w, Vec<float, N> move, float decay) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) w[k] -= __builtin_fmaf(decay, w[k], move[k]);
     return w;
 }
 
-// One piece a workgroup, N elements a lane: everything is asked for before anything is used.
-template <int N, typename P, typename G, bool MASTER>
+enum { kWeights = 0, kMasters = 1, kMoves = 2 };   // where a step's moves go
+
+// One piece a workgroup, four elements a lane: everything is asked for before anything is used.
+template <typename P, typename G, int TO>
 __global__ __launch_bounds__(kBlock) void adamw32_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
-    const Piece c = piece_of<N == 4 ? kFine : kWide>(ps);
+    const Piece c = piece_of<kFine>(ps);
     const G* g = grad_of<G>(c, ga);
-    if (!g || (a.skip && *a.skip)) return;
+    const bool skip = a.skip && *a.skip;
+    if (!g || (TO != kMoves && skip)) return;
     const AdamwRates r = a.device_rates ? *a.device_rates : a.rates;
     const float f = factor_of(c, a.coefs, a.per_tensor, a.scale);
     P* p = static_cast<P*>(c.t.param) + c.at;
-    float *pm = static_cast<float*>(c.t.m) + c.at, *pv = static_cast<float*>(c.t.v) + c.at, *pw = c.t.master + c.at;
-    const int i = threadIdx.x * N, k = c.n - i;
+    float *pm = static_cast<float*>(c.t.m) + c.at, *pv = static_cast<float*>(c.t.v) + c.at;
+    float* pw = TO == kMoves ? a.moves + c.t.flat + c.at : c.t.master + c.at;
+    const int i = threadIdx.x * 4, k = c.n - i;
     if (k <= 0) return;
-    by_length<kBlock * N>(c, [&](auto full) {
+    by_length<kBlock * 4>(c, [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        const Vec<G, N> gx = load_some<N, FULL>(g + i, k);
-        Vec<float, N> m = load_some<N, FULL>(pm + i, k), v = load_some<N, FULL>(pv + i, k), w;
-        if constexpr (MASTER) w = load_some<N, FULL>(pw + i, k);
-        else w = to_float<N>(load_some<N, FULL>(p + i, k));
-        moments<N>(to_float<N>(gx) * f, a, m, v);
-        w = weights<N>(w, m, v, a, r);
-        store_some<N, FULL>(pm + i, m, k);
-        store_some<N, FULL>(pv + i, v, k);
-        if constexpr (MASTER) store_some<N, FULL>(pw + i, w, k);
-        store_some<N, FULL>(p + i, from_float<P, N>(w), k);
+        if constexpr (TO == kMoves)
+            if (skip) return store_some<4, FULL>(pw + i, Vec<float, 4>{}, k);
+        const Vec<G, 4> gx = load_some<4, FULL>(g + i, k);
+        Vec<float, 4> m = load_some<4, FULL>(pm + i, k), v = load_some<4, FULL>(pv + i, k), w;
+        if constexpr (TO == kMasters) w = load_some<4, FULL>(pw + i, k);
+        if constexpr (TO == kWeights) w = to_float<4>(load_some<4, FULL>(p + i, k));
+        moments<4>(to_float<4>(gx) * f, a, m, v);
+        const Vec<float, 4> move = moves_of<4>(m, v, a, r);
+        store_some<4, FULL>(pm + i, m, k);
+        store_some<4, FULL>(pv + i, v, k);
+        if constexpr (TO == kMoves) return store_some<4, FULL>(pw + i, move, k);
+        w = moved<4>(w, move, r.decay);
+        if constexpr (TO == kMasters) store_some<4, FULL>(pw + i, w, k);
+        store_some<4, FULL>(p + i, from_float<P, 4>(w), k);
+    });
+}
+
+// The other half of a step whose moves went through the exchange.
+template <typename P, bool MASTER>
+__global__ __launch_bounds__(kBlock) void apply_kernel(Pieces ps, const float* __restrict__ moves, float scale, float decay,
+                                                       const float* __restrict__ lr, float weight_decay) {
+    const Piece c = piece_of<kFine>(ps);
+    if (lr) decay = *lr * weight_decay;
+    P* p = static_cast<P*>(c.t.param) + c.at;
+    float* pw = c.t.master + c.at;
+    const int i = threadIdx.x * 4, k = c.n - i;
+    if (k <= 0) return;
+    by_length<kBlock * 4>(c, [&](auto full) {
+        constexpr bool FULL = decltype(full)::value;
+        const Vec<float, 4> move = load_some<4, FULL>(moves + c.t.flat + c.at + i, k);
+        Vec<float, 4> w;
+        if constexpr (MASTER) w = load_some<4, FULL>(pw + i, k);
+        else w = to_float<4>(load_some<4, FULL>(p + i, k));
+        w = moved<4>(w, move * scale, decay);
+        if constexpr (MASTER) store_some<4, FULL>(pw + i, w, k);
+        store_some<4, FULL>(p + i, from_float<P, 4>(w), k);
     });
 }
 
@@ -244,11 +281,12 @@ __device__ __forceinline__ void store_states(const Eight<SPLIT, FULL>& e, Vec<fl
         global(of_v ? sv : sm)[b] = kept ? (of_v ? top : top * (float)(1.0 / 448.0)) : 0.0f;
 }
 
-template <typename P, typename G, bool MASTER>
+template <typename P, typename G, int TO>
 __global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
     const Piece c = piece_of<kWide>(ps);
     const G* g = grad_of<G>(c, ga);
-    if (!g || (a.skip && *a.skip)) return;
+    const bool skip = a.skip && *a.skip;
+    if (!g || (TO != kMoves && skip)) return;
     const AdamwRates r = a.device_rates ? *a.device_rates : a.rates;
     const float f = factor_of(c, a.coefs, a.per_tensor, a.scale);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -256,24 +294,28 @@ __global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, 
     if (blocks <= 0) return;
     P* p = static_cast<P*>(c.t.param) + c.at;
     unsigned char *pm = static_cast<unsigned char*>(c.t.m) + c.at, *pv = static_cast<unsigned char*>(c.t.v) + c.at;
-    float* pw = c.t.master + c.at;
+    float* pw = TO == kMoves ? a.moves + c.t.flat + c.at : c.t.master + c.at;
     const long long block = c.at / CX_STATE_BLOCK + wave * 2;
     float *sm = c.t.m_scale + block, *sv = c.t.v_scale + block;
     by_length<kBlock * 8>(c, [&](auto full) {
         constexpr bool FULL = decltype(full)::value;
-        constexpr bool SPLIT = MASTER || sizeof(P) == 4 || sizeof(G) == 4;
+        constexpr bool SPLIT = TO != kWeights || sizeof(P) == 4 || sizeof(G) == 4;
         const Eight<SPLIT, FULL> e(c.n);
+        if constexpr (TO == kMoves)
+            if (skip) return e.store(pw, Vec<float, 8>{});
         const Vec<G, 8> gx = e.load(g);
         const Codes mc = __builtin_bit_cast(Codes, e.load(pm)), vc = __builtin_bit_cast(Codes, e.load(pv));
         Vec<float, 8> w;
-        if constexpr (MASTER) w = e.load(pw);
-        else w = to_float<8>(e.load(p));
+        if constexpr (TO == kMasters) w = e.load(pw);
+        if constexpr (TO == kWeights) w = to_float<8>(e.load(p));
         const int mine = FULL || blocks > 1 ? (threadIdx.x >> 5) & 1 : 0;
         Vec<float, 8> m = m_value(mc, global(sm)[mine]), v = v_value(vc, global(sv)[mine]);
         moments<8>(to_float<8>(gx) * f, a, m, v);
-        w = weights<8>(w, m, v, a, r);
-        if constexpr (MASTER) e.store(pw, w);
-        e.store(p, from_float<P, 8>(w));
+        const Vec<float, 8> move = moves_of<8>(m, v, a, r);
+        if constexpr (TO != kMoves) w = moved<8>(w, move, r.decay);
+        if constexpr (TO == kMoves) e.store(pw, move);
+        if constexpr (TO == kMasters) e.store(pw, w);
+        if constexpr (TO != kMoves) e.store(p, from_float<P, 8>(w));
         store_states(e, m, v, pm, pv, sm, sv, blocks);
     });
 }
@@ -305,17 +347,17 @@ __global__ __launch_bounds__(kBlock) void set_states_kernel(Pieces ps, const flo
                  static_cast<unsigned char*>(c.t.v) + c.at, c.t.m_scale + block, c.t.v_scale + block, blocks);
 }
 
-template <typename P, typename G, bool MASTER>
+template <typename P, typename G, int TO>
 void launch_step(hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
-    if (bits == 32) adamw32_kernel<4, P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
-    else adamw8_kernel<P, G, MASTER><<<n, kBlock, 0, s>>>(ps, g, a);
+    if (bits == 32) adamw32_kernel<P, G, TO><<<n, kBlock, 0, s>>>(ps, g, a);
+    else adamw8_kernel<P, G, TO><<<n, kBlock, 0, s>>>(ps, g, a);
 }
 
-template <typename P, bool MASTER>
+template <typename P, int TO>
 void launch_step_for(int grad_type, hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
-    if (grad_type == CX_F32) launch_step<P, float, MASTER>(s, bits, n, ps, g, a);
-    else if (grad_type == CX_BF16) launch_step<P, __bf16, MASTER>(s, bits, n, ps, g, a);
-    else launch_step<P, _Float16, MASTER>(s, bits, n, ps, g, a);
+    if (grad_type == CX_F32) launch_step<P, float, TO>(s, bits, n, ps, g, a);
+    else if (grad_type == CX_BF16) launch_step<P, __bf16, TO>(s, bits, n, ps, g, a);
+    else launch_step<P, _Float16, TO>(s, bits, n, ps, g, a);
 }
 
 }  // namespace
@@ -331,6 +373,7 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
     a.coefs = u->n_coefs ? u->d_coefs : nullptr;
     a.per_tensor = u->n_coefs != 1;
     a.skip = u->d_skip;
+    a.moves = u->d_moves;
     if (u->d_step || u->d_lr) {
         AdamwRates* rates = reinterpret_cast<AdamwRates*>(t->d_rates);
         rates_kernel<<<1, 1, 0, h->stream>>>(u->d_step, u->step, u->d_lr, u->lr, u->beta1, u->beta2, u->weight_decay,
@@ -342,14 +385,32 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
     }
     return for_grads(t, g, t->state_bits == 32 ? kFine : kWide, [&](const Pieces& ps, int n, const GradArgs& ga) -> int {
         const int bits = t->state_bits;
-        if (t->param_type == CX_F32) launch_step_for<float, false>(g->type, h->stream, bits, n, ps, ga, a);
-        else if (t->param_type == CX_BF16 && t->masters) launch_step_for<__bf16, true>(g->type, h->stream, bits, n, ps, ga, a);
-        else if (t->param_type == CX_BF16) launch_step_for<__bf16, false>(g->type, h->stream, bits, n, ps, ga, a);
-        else if (t->masters) launch_step_for<_Float16, true>(g->type, h->stream, bits, n, ps, ga, a);
-        else launch_step_for<_Float16, false>(g->type, h->stream, bits, n, ps, ga, a);
+        hipStream_t s = h->stream;
+        if (u->d_moves) launch_step_for<float, kMoves>(g->type, s, bits, n, ps, ga, a);  // (no weights: no type of theirs)
+        else if (t->param_type == CX_F32) launch_step_for<float, kWeights>(g->type, s, bits, n, ps, ga, a);
+        else if (t->param_type == CX_BF16 && t->masters) launch_step_for<__bf16, kMasters>(g->type, s, bits, n, ps, ga, a);
+        else if (t->param_type == CX_BF16) launch_step_for<__bf16, kWeights>(g->type, s, bits, n, ps, ga, a);
+        else if (t->masters) launch_step_for<_Float16, kMasters>(g->type, s, bits, n, ps, ga, a);
+        else launch_step_for<_Float16, kWeights>(g->type, s, bits, n, ps, ga, a);
         CX_HIP(hipGetLastError());
         return CX_OK;
     });
+}
+
+int launch_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, float scale, double lr, const float* d_lr,
+                       double weight_decay) {
+    const int n = t->cut[kFine].pieces;
+    if (n == 0) return CX_OK;
+    const Pieces ps = t->pieces(kFine);
+    const float decay = (float)(lr * weight_decay), wd = (float)weight_decay;
+    hipStream_t s = h->stream;
+    if (t->param_type == CX_F32) apply_kernel<float, false><<<n, kBlock, 0, s>>>(ps, d_moves, scale, decay, d_lr, wd);
+    else if (t->param_type == CX_BF16 && t->masters) apply_kernel<__bf16, true><<<n, kBlock, 0, s>>>(ps, d_moves, scale, decay, d_lr, wd);
+    else if (t->param_type == CX_BF16) apply_kernel<__bf16, false><<<n, kBlock, 0, s>>>(ps, d_moves, scale, decay, d_lr, wd);
+    else if (t->masters) apply_kernel<_Float16, true><<<n, kBlock, 0, s>>>(ps, d_moves, scale, decay, d_lr, wd);
+    else apply_kernel<_Float16, false><<<n, kBlock, 0, s>>>(ps, d_moves, scale, decay, d_lr, wd);
+    CX_HIP(hipGetLastError());
+    return CX_OK;
 }
 
 int launch_adamw_states(cx_handle h, cx_tensors t, int dt, void* d_m, void* d_v) {

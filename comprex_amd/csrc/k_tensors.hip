@@ -385,10 +385,27 @@ int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_ada
     if (!(a->weight_decay >= 0.0 && std::isfinite(a->weight_decay)))
         return fail(CX_ERR_INVALID, "cx_adamw_step: the weight decay must be finite and not negative");
     if (!std::isfinite(a->scale)) return fail(CX_ERR_INVALID, "cx_adamw_step: scale must be finite");
+    if (!aligned_to(a->d_moves, 4)) return fail(CX_ERR_INVALID, "cx_adamw_step: misaligned moves");
     if (!a->d_step && a->step < 1) return fail(CX_ERR_INVALID, "cx_adamw_step: steps count from 1");
     DeviceScope on(t->device);
     CX_HIP(on.error);
     return launch_adamw(h, t, grads, a);
+}
+
+int cx_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, double scale, double lr, const float* d_lr,
+                   double weight_decay) {
+    const int rc = check_set(h, t, "cx_adamw_apply");
+    if (rc != CX_OK) return rc;
+    if (!t->adamw) return fail(CX_ERR_INVALID, "cx_adamw_apply: the set was made without a state");
+    if ((!d_moves && t->total > 0) || !aligned_to(d_moves, 4))
+        return fail(CX_ERR_INVALID, "cx_adamw_apply: null or misaligned moves");
+    if (!d_lr && !(lr >= 0.0 && std::isfinite(lr)))
+        return fail(CX_ERR_INVALID, "cx_adamw_apply: the learning rate must be finite and not negative");
+    if (!(weight_decay >= 0.0 && std::isfinite(weight_decay)) || !std::isfinite(scale))
+        return fail(CX_ERR_INVALID, "cx_adamw_apply: weight decay and scale must be finite, the former not negative");
+    DeviceScope on(t->device);
+    CX_HIP(on.error);
+    return launch_adamw_apply(h, t, d_moves, (float)scale, lr, d_lr, weight_decay);
 }
 
 int cx_adamw_states(cx_handle h, cx_tensors t, cx_dtype dt, void* d_exp_avg, void* d_exp_avg_sq) {

@@ -244,6 +244,12 @@ class Handle:
         allocate (cx_reserve)."""
         check(self.lib.cx_reserve(self._h, _DT[dtype], int(n), int(paths)))
 
+    def set_stream(self, stream):
+        """Works on another stream from now on (waits for the one before, if it is another)."""
+        if stream.cuda_stream != self.stream.cuda_stream:
+            check(self.lib.cx_set_stream(self._h, C.c_void_p(stream.cuda_stream)))
+        self.stream = stream
+
     def set_option(self, key, value):
         check(self.lib.cx_set_option(self._h, key.encode(), int(value)))
 
@@ -433,11 +439,13 @@ class Handle:
         return out
 
     def adamw_step(self, tensors, grads, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, coefs=None, scale=1.0,
-                   skip=None):
+                   skip=None, moves=None):
         """One AdamW step on an AdamWSet with the gradients times coefs and scale (cx_adamw_step).  `grads`: a
         list (None: leave this tensor alone) or the flat vector; `step`: which step this is, from 1, or an int32
         device tensor that the call advances; `lr`: a number or an fp32 device tensor; `skip` (int32) other than
-        0: nothing changes."""
+        0: nothing changes.  With `moves`, a flat fp32 vector, the moments take the step and what the weights would
+        lose goes there, for an exchange between ranks and `adamw_apply` (a tensor without a gradient: its part is
+        left as it is; skipped: zeros)."""
         g = tensors.gradients(grads)
         on_device = isinstance(step, torch.Tensor)
         d_lr = isinstance(lr, torch.Tensor)
@@ -445,7 +453,18 @@ class Handle:
         check(self.lib.cx_adamw_step(self._h, tensors._t, g, _lib.AdamwArgs(
             0.0 if d_lr else lr, betas[0], betas[1], eps, weight_decay, scale, 0 if on_device else step,
             tensors._one(step, torch.int32, "step") if on_device else None,
-            tensors._one(lr, torch.float32, "lr") if d_lr else None, at, n, tensors._one(skip, torch.int32, "skip"))))
+            tensors._one(lr, torch.float32, "lr") if d_lr else None, at, n, tensors._one(skip, torch.int32, "skip"),
+            None if moves is None else tensors._vector(moves, torch.float32, "moves").data_ptr())))
+
+    def adamw_apply(self, tensors, moves, lr, weight_decay=0.01, scale=1.0):
+        """The weights of an AdamWSet after `scale` times the flat vector of moves (adamw_step) and the decay:
+        w (1 - lr weight_decay) - scale moves."""
+        if moves is None:
+            raise _invalid("needs the moves")
+        d_lr = isinstance(lr, torch.Tensor)
+        check(self.lib.cx_adamw_apply(self._h, tensors._t, tensors._vector(moves, torch.float32, "moves").data_ptr(), scale,
+                                      0.0 if d_lr else lr, tensors._one(lr, torch.float32, "lr") if d_lr else None,
+                                      weight_decay))
 
     def adamw_states(self, tensors, dtype=torch.float32, exp_avg=None, exp_avg_sq=None):
         """What the 8-bit moments of an AdamWSet stand for: (exp_avg, exp_avg_sq), flat vectors of `dtype`."""

@@ -1,5 +1,8 @@
-"""PyTorch counterpart of the reference's Keras optimizer (keras/comprex_optimizer.py:7-170):
-momentum SGD whose gradient exchange is one of the compressed allreduce schedules.
+"""Optimizers whose gradient exchange is one of the compressed allreduce schedules: `ComprexOptimizer` (momentum
+SGD) and `ComprexAdamW`.
+
+`ComprexOptimizer` is the PyTorch counterpart of the reference's Keras optimizer
+(keras/comprex_optimizer.py:7-170):
 
 Per step and rank (blob mode, keras/comprex_optimizer.py:97-133): every gradient is clipped to
 `pre_clipnorm`, turned into a local momentum term `m = momentum * m + lr * g`, all terms are
@@ -7,16 +10,32 @@ concatenated into ONE flat device buffer, the allreduce works in place on that b
 pointer handed straight to the C ABI), the result is divided by the number of ranks, and
 `w = (1 - weight_decay) * w - avg_m`.  With a single rank nothing is exchanged and, as in the
 reference (:134-141,155-163), the update is `m = momentum * m + g; w = (1 - wd) * w - m`.
+
+`ComprexAdamW` has no counterpart in the reference and keeps its order: every rank's moments follow its own
+gradients (clipped together), what its weights would lose to the step is exchanged, and every rank applies the
+average.  The schedules deliver each rank another vector and make up for it later; sums bear that, moments of
+such vectors would not and the ranks' weights would drift apart.  Clipping and the step run as a few launches
+over all tensors (`Handle.grad_norms`, `adamw_step`, `adamw_apply`), and nothing waits for the device.
 """
 import torch
 
 from . import pygpi
+from .device import AdamWSet, Handle
 
 _SCHEDULES = {
     "comprex_alltoone": pygpi.Comprex_AllToOneAllreduce,
     "comprex_ring": pygpi.Comprex_RingAllreduce,
     "comprex_bigring": pygpi.Comprex_BigRingAllreduce,
 }
+
+
+def _make_allreduce(kind, gaspi_env, size, compression_ratio, size_factor):
+    ar = _SCHEDULES[kind](gaspi_env)
+    if kind == "comprex_alltoone":
+        ar.setup_connections(size, 1, 0, compression_ratio, size_factor)
+    else:
+        ar.setup_connections(size, 1, compression_ratio, size_factor)
+    return ar
 
 
 class ComprexOptimizer(torch.optim.Optimizer):
@@ -41,12 +60,7 @@ class ComprexOptimizer(torch.optim.Optimizer):
             self.allreduce.set_compression_ratio(compression_ratio)
 
     def _create_allreduce(self, size):
-        ar = _SCHEDULES[self.allreduce_type](self.gaspi_env)
-        if self.allreduce_type == "comprex_alltoone":
-            ar.setup_connections(size, 1, 0, self.compression_ratio, self.size_factor)
-        else:
-            ar.setup_connections(size, 1, self.compression_ratio, self.size_factor)
-        return ar
+        return _make_allreduce(self.allreduce_type, self.gaspi_env, size, self.compression_ratio, self.size_factor)
 
     @torch.no_grad()
     def step(self):
@@ -84,3 +98,223 @@ class ComprexOptimizer(torch.optim.Optimizer):
         for p, group, _ in entries:
             p.mul_(1 - group["weight_decay"]).sub_(self.blob[off:off + p.numel()].view_as(p))
             off += p.numel()
+
+
+class _Part:
+    """The parameters of one group that share a type and a width of the moments, and their AdamWSet."""
+
+    def __init__(self, group, params):
+        self.group, self.params = group, params
+        self.set = self.made_of = self.count = None
+
+    def tensors(self, state):
+        """params, exp_avg, exp_avg_sq, masters, scales of both: lists, or None."""
+        states = [state[p] for p in self.params]
+        return [self.params] + [[s[k] for s in states] if k in states[0] else None
+                                for k in ("exp_avg", "exp_avg_sq", "master", "exp_avg_scales", "exp_avg_sq_scales")]
+
+
+class ComprexAdamW(torch.optim.Optimizer):
+    """AdamW over the compressed allreduce.
+
+    Per step and rank: the gradients are clipped together to the norm `clip_norm` (None: not at all) and the
+    moments take them.  With one rank the weights follow at once.  With several, the moves of all weights go as one
+    flat fp32 vector through the exchange and come back summed, and every weight takes a `1 / ranks` of its sum
+    and its decay; one without a gradient here may have had one elsewhere.
+
+    state_bits 8: the moments of parameters of at least `min_8bit_size` elements take one byte each.
+    master_weights: bf16 and fp16 parameters get fp32 weights of which they are the rounded values.
+    skip_nonfinite: a gradient with an infinity or NaN anywhere leaves its rank's moments and count as they are,
+    and its weights too or, with several ranks, its part of the sum zero; decided on the device, where the steps
+    are counted then (a parameter without a gradient counts along with those it is stepped with).  Parameters are contiguous and on one GPU."""
+
+    def __init__(self, params, gaspi_env, learning_rate=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
+                 clip_norm=None, state_bits=32, min_8bit_size=4096, master_weights=True, skip_nonfinite=False,
+                 compression_ratio=0.01, allreduce_type="comprex_bigring", size_factor=1.0):
+        if allreduce_type not in _SCHEDULES:
+            raise ValueError("AllreduceOp with name %s is not known!" % allreduce_type)
+        if state_bits not in (8, 32):
+            raise ValueError("`state_bits` must be 8 or 32.")
+        if clip_norm is not None and not clip_norm > 0:
+            raise ValueError("`clip_norm` must be above 0.")
+        if not all(0 <= b < 1 for b in betas):
+            raise ValueError("`betas` must be in [0, 1).")
+        super().__init__(params, dict(lr=learning_rate, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        for group in self.param_groups:
+            for p in group["params"]:
+                self._check(p)
+        self.gaspi_env = gaspi_env
+        self.clip_norm, self.state_bits, self.min_8bit_size = clip_norm, state_bits, min_8bit_size
+        self.master_weights, self.skip_nonfinite = master_weights, skip_nonfinite
+        self.compression_ratio, self.allreduce_type, self.size_factor = compression_ratio, allreduce_type, size_factor
+        self.handle = self.allreduce = self.blob = self._parts = None
+        self._exchange_stream = None
+
+    @staticmethod
+    def _check(p):
+        if not p.is_cuda or not p.is_contiguous() or p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+            raise ValueError("parameters are contiguous fp32, bf16 or fp16 tensors on a GPU")
+
+    def set_compression_ratio(self, compression_ratio):
+        self.compression_ratio = compression_ratio
+        if self.allreduce is not None:
+            self.allreduce.set_compression_ratio(compression_ratio)
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        self._sync_counts()
+        self._parts = None
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # the base class casts a parameter's state to the parameter's type: taken once more as it was saved
+        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(ids, params):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                 for k, v in state_dict["state"][i].items()}
+        self._parts = None
+
+    def _new_state(self, p):
+        state = self.state[p]
+        state["step"] = 0
+        if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
+            (state["exp_avg"], state["exp_avg_sq"], state["exp_avg_scales"],
+             state["exp_avg_sq_scales"]) = AdamWSet.zeros8(p)
+        else:
+            state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+            state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        if self.master_weights and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32)
+
+    def _make_parts(self):
+        parts = {}
+        for k, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                if not p.requires_grad:
+                    continue
+                self._check(p)
+                if "exp_avg" not in self.state[p]:
+                    self._new_state(p)
+                key = (k, p.dtype, "exp_avg_scales" in self.state[p], "master" in self.state[p])
+                parts.setdefault(key, _Part(group, [])).params.append(p)
+        self._parts = list(parts.values())
+
+    def _sync_counts(self):
+        """The steps' counts where they live on the device, into the state (a saved state holds numbers)."""
+        for part in getattr(self, "_parts", None) or ():
+            if part.count is not None:
+                n = int(part.count)
+                for p in part.params:
+                    self.state[p]["step"] = n
+
+    def state_dict(self):
+        self._sync_counts()
+        return super().state_dict()
+
+    def _make_sets(self):
+        """The parts' sets, made anew where a tensor has moved (a state that was replaced, a model that was)."""
+        stream = torch.cuda.current_stream(self._parts[0].params[0].device)
+        if self.handle is None or self.handle.device != stream.device:
+            with torch.cuda.device(stream.device):
+                self.handle = Handle(stream)
+            for part in self._parts:
+                part.set = None
+        self.handle.set_stream(stream)
+        for part in self._parts:
+            lists = part.tensors(self.state)
+            now = [t.data_ptr() for x in lists if x is not None for t in x]
+            if part.set is None or part.made_of != now:
+                part.set, part.made_of = AdamWSet(self.handle, *lists), now
+                if self.skip_nonfinite and part.count is None:
+                    part.count = torch.full((1,), self.state[part.params[0]]["step"], dtype=torch.int32,
+                                            device=stream.device)
+        return stream
+
+    def _grads(self, part):
+        grads = [p.grad for p in part.params]
+        for k, g in enumerate(grads):
+            if g is None:
+                continue
+            if g.is_sparse:
+                raise RuntimeError("ComprexAdamW takes dense gradients only")
+            if not g.is_contiguous():
+                grads[k] = g.contiguous()
+        return grads
+
+    def _clip(self, live):
+        """(coefficient or None, non-finite flag or None) of all gradients together."""
+        if not live or (self.clip_norm is None and not self.skip_nonfinite):
+            return None, None
+        found = [self.handle.grad_norms(part.set, g, self.clip_norm if len(live) == 1 else None) for part, g in live]
+        if len(found) == 1:
+            norms, coef, flag = found[0]
+        else:
+            norm = torch.linalg.vector_norm(torch.stack([f[0][-1] for f in found]).double())
+            coef = None
+            if self.clip_norm is not None:
+                coef = torch.where(norm > self.clip_norm, self.clip_norm / norm, 1.0).float().reshape(1)
+            flag = torch.stack([f[2] for f in found]).amax(0)
+        return (coef if self.clip_norm is not None else None), (flag if self.skip_nonfinite else None)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        ranks = self.gaspi_env.get_ranks()
+        if self._parts is None:
+            self._make_parts()
+        if not self._parts:
+            return loss
+        stream = self._make_sets()
+        parts, lists = self._parts, [self._grads(part) for part in self._parts]
+        ready = [part.set.gradients(g) if any(x is not None for x in g) else None for part, g in zip(parts, lists)]
+        coef, flag = self._clip([(part, g) for part, g in zip(parts, ready) if g is not None])
+        if ranks == 1:
+            for part, g, checked in zip(parts, lists, ready):
+                if checked is not None:
+                    self._step_part(part, g, checked, coef, flag)
+            return loss
+        total = sum(part.set.total for part in parts)
+        if self.blob is None or self.blob.numel() != total:
+            self.blob = torch.empty(total, dtype=torch.float32, device=stream.device)
+            self.allreduce = _make_allreduce(self.allreduce_type, self.gaspi_env, total, self.compression_ratio,
+                                             self.size_factor)
+        at = 0
+        for part, g, checked in zip(parts, lists, ready):
+            moves = self.blob[at:at + part.set.total]
+            if any(x is None for x in g):
+                moves.zero_()
+            if checked is not None:
+                self._step_part(part, g, checked, coef, flag, moves)
+            at += part.set.total
+        if stream.cuda_stream != (self._exchange_stream or 0):  # the exchange orders itself with this stream
+            self.gaspi_env.set_user_stream(stream)
+            self._exchange_stream = stream.cuda_stream
+        self.allreduce.apply(self.blob)  # in place, on the device
+        at = 0
+        for part in parts:
+            self.handle.adamw_apply(part.set, self.blob[at:at + part.set.total], part.group["lr"],
+                                    part.group["weight_decay"], scale=1.0 / ranks)
+            at += part.set.total
+        return loss
+
+    def _step_part(self, part, grads, checked, coef, flag, moves=None):
+        """The step of a part's parameters that have a gradient (`checked`: the same, ready for the set)."""
+        group = part.group
+        how = dict(betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], coefs=coef, skip=flag,
+                   moves=moves)
+        if part.count is not None:
+            self.handle.adamw_step(part.set, checked, part.count, group["lr"], **how)
+            return
+        states = [self.state[p] for p in part.params]
+        for s, g in zip(states, grads):
+            if g is not None:
+                s["step"] += 1
+        counts = sorted({s["step"] for s, g in zip(states, grads) if g is not None})
+        for n in counts:  # one, unless some parameter went without a gradient before
+            these = checked if len(counts) == 1 else [g if s["step"] == n else None for s, g in zip(states, grads)]
+            self.handle.adamw_step(part.set, these, n, group["lr"], **how)

@@ -375,7 +375,14 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
  * under the root); the parameter is w rounded once, 8-bit states are m and v rounded after w took them.
  * step >= 1 counts this step.  With d_step (device int) the count lives on the device: the call adds 1 to
  * it and uses the result; `step` is ignored.  d_lr (device float) replaces lr.  *d_skip != 0 leaves
- * everything as it is, *d_step too. */
+ * everything as it is, *d_step too.
+ *
+ * d_moves != NULL: only the moments take the step, and what w would lose to it, lr / (1 - beta1^step) * m / (...),
+ * goes to this flat fp32 vector (the tensors back to back; *d_skip != 0: zeros; a tensor without a gradient: left
+ * as it is) for the exchange to sum.  Ranks whose vectors differ for a while, as the compressed schedules leave
+ * them, end up with the same weights that way (sums are delivered late, never lost), as they do with the momentum
+ * terms of keras/comprex_optimizer.py:97-133; moments of their own of differing sums would drift apart.
+ * cx_adamw_apply is the other half: w = w (1 - lr weight_decay) - scale * moves, for every tensor of the set. */
 typedef struct {
     double lr, beta1, beta2, eps, weight_decay, scale;
     long long step;
@@ -384,8 +391,11 @@ typedef struct {
     const float* d_coefs;
     int n_coefs;               /* 0, 1 or the set's count */
     const int* d_skip;
+    float* d_moves;
 } cx_adamw_args;
 int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* args);
+int cx_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, double scale, double lr, const float* d_lr,
+                   double weight_decay);
 
 /* The values that the 8-bit states of a set stand for, all tensors back to back (dt: CX_F32, CX_BF16 or
  * CX_F16), and back: states from values (fp32).  For checkpoints that hold 32 bits. */

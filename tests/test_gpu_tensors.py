@@ -374,6 +374,71 @@ def test_adamw_count_and_rate_on_the_device(bits):
         assert same(A.snapshot(), B.snapshot())
 
 
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("param,grad,master", TYPES, ids=str)
+def test_adamw_moves_and_apply_are_the_step(param, grad, master, bits, offset):
+    """The step in two halves, moves and weights, has the bits of the step in one."""
+    sizes = [1, 257, 70001, 0, 1024, 2048, 100]
+    A, B = (Params(10, sizes, param, bits, master, offset) for _ in range(2))
+    moves = odd(np.full(sum(sizes), 7.0), F32, offset)
+    count, skip = (torch.zeros(1, dtype=torch.int32, device="cuda") for _ in range(2))
+    coef = torch.full((1,), 0.3, device="cuda")
+    for step in (1, 2, 3):
+        grads, scale = A.gradients(grad, offset)
+        if step == 2:  # nothing but zeros comes out of a step that is skipped
+            was = B.snapshot()
+            skip.fill_(1)
+            B.h.adamw_step(B.set, grads, count, 1e-2, coefs=coef, scale=scale, skip=skip, moves=moves)
+            assert moves.count_nonzero() == 0 and same(was, B.snapshot()) and count.item() == 1
+            skip.zero_()
+        A.h.adamw_step(A.set, grads, step, 1e-2, weight_decay=0.2, coefs=coef, scale=scale)
+        w = [None if x is None else [t.clone() for t in x] for x in (B.p, B.w)]
+        B.h.adamw_step(B.set, grads, count, 1e-2, weight_decay=0.2, coefs=coef, scale=scale, skip=skip, moves=moves)
+        assert same(w, (B.p, B.w))  # the weights wait for the other half
+        B.h.adamw_apply(B.set, moves, 1e-2, 0.2)
+        assert same(A.snapshot(), B.snapshot())
+    # without a gradient: its part of the moves is left
+    moves.fill_(5.0)
+    grads[2] = None
+    B.h.adamw_step(B.set, grads, 4, 1e-2, scale=scale, moves=moves)
+    assert (moves[258:258 + 70001] == 5).all() and not (moves[258 + 70001:] == 5).any() and not (moves[:258] == 5).any()
+    # a scale, and a rate on the device
+    w = f64((B.w or B.p)[2])
+    B.h.adamw_apply(B.set, moves, torch.full((1,), 0.5, device="cuda"), 0.25, scale=-0.5)
+    want = w - 0.125 * w + 2.5
+    last = 0.0 if param == F32 or master else half_step(param, want) * 1.01
+    assert (np.abs(f64((B.w or B.p)[2]) - want) <= 3 * U * (np.abs(w) + 3) + last).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_packed_gradients_through_the_codec_and_into_a_step(dtype):
+    """As one channel of the exchange uses them: clipped and packed, written with error feedback, added on the other
+    side, taken by a step.  What a message does not carry stays in the residual, bit for bit."""
+    D = device_module()
+    sizes = [5000, 3, 70001, 256]
+    P = Params(11, sizes, F32, 32, False, 0)
+    total = sum(sizes)
+    rests, flat, got = (torch.zeros(total, device="cuda") for _ in range(3))
+    msg = torch.zeros(D.message_capacity(total, F32), dtype=torch.uint8, device="cuda")
+    for step in (1, 2, 3):
+        grads, _ = P.gradients(F32, 0)
+        grads = [g.to(dtype) for g in grads]
+        norms, coefs, flag = P.h.grad_norms(P.set, grads, 0.1)
+        P.h.pack(P.set, grads, out=flat, coefs=coefs, skip=flag)
+        want = torch.cat([g.float() * coefs for g in grads])
+        assert torch.equal(flat, want)
+        owed = rests + flat
+        P.h.write_step(msg, flat, rests, 0.05, sync=False)
+        got.zero_()
+        P.h.add(got, msg)
+        assert torch.equal(got + rests, owed) and 0 < int(got.count_nonzero()) < total
+        before = P.now()
+        P.h.adamw_step(P.set, got, step, 1e-3, scale=0.5)
+        check_step(P, before, [f64(g) for g in got.split(sizes)], [0.5] * 4, step, 1e-3, 0.9, 0.999, 1e-8, 0.01)
+    P.h.synchronize()
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_nonfinite_elements_stay_alone(bits):
     """Without a skip an infinity or NaN ruins its own weight and nothing else."""
@@ -516,6 +581,13 @@ def test_refusals_on_the_device():
     refused(bad, h.adamw_step, s, [g], 1, 1e-3, weight_decay=-1.0)
     refused(bad, h.adamw_step, s, [g], 1, 1e-3, scale=math.inf)
     refused(size, h.adamw_step, s, [g], 1, 1e-3, coefs=torch.ones(2, device="cuda"))
+    refused(bad, h.adamw_step, s, [g], 1, 1e-3, moves=torch.zeros(10, dtype=BF16, device="cuda"))
+    refused(size, h.adamw_step, s, [g], 1, 1e-3, moves=torch.zeros(11, device="cuda"))
+    refused(bad, h.adamw_apply, s, None, 1e-3)
+    refused(bad, h.adamw_apply, plain, z(), 1e-3)
+    refused(bad, h.adamw_apply, s, z(), -1.0)
+    refused(bad, h.adamw_apply, s, z(), 1e-3, weight_decay=math.nan)
+    refused(bad, h.adamw_apply, s, z(), 1e-3, scale=math.inf)
     refused(bad, h.grad_norms, s, [g], 0.0)
     refused(bad, h.grad_norms, s, [g], math.nan)
     # the output across the gradients, in a place that is not their own

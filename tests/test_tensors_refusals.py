@@ -142,7 +142,7 @@ def test_c_entry_point_checks_before_it_touches_a_device():
     assert L.cx_tensors_destroy(None) == 0
     for rc in (L.cx_grad_norms(None, None, None, 1.0, 1.0, 0, None, None, None),
                L.cx_pack(None, None, None, None, 0, 1.0, None, None), L.cx_adamw_step(None, None, None, None),
-               L.cx_adamw_states(None, None, 0, None, None), L.cx_adamw_set_states(None, None, None, None)):
+               L.cx_adamw_apply(None, None, None, 1.0, 1.0, None, 0.0), L.cx_adamw_states(None, None, 0, None, None), L.cx_adamw_set_states(None, None, None, None)):
         assert rc == bad
     if _lib.lib().cx_device_count() == 0:
         assert create(1, one, state()) == _lib.CX_ERR_HIP                           # sound, but there is no device
