@@ -178,6 +178,7 @@ struct cx_tensors_s {
     // device
     cx::Tensor* d_tensors = nullptr;
     double* d_partial = nullptr;            // per coarse piece: sum of the gradient's squares
+    unsigned* d_done = nullptr;             // workgroups of small_norms_kernel that are through; 0 between launches
     float* d_rates = nullptr;               // what a device-side step count gives (AdamwRates)
 
     cx::Pieces pieces(int which, int from = 0) const {

@@ -36,11 +36,8 @@ __device__ __forceinline__ double add_squares(double s, Vec<float, 4> x) {
     return s;
 }
 
-// partial[piece] = sum of g^2.  64 bits: the squares of finite floats do not overflow there.
-template <typename G>
-__global__ __launch_bounds__(kBlock) void squares_kernel(Pieces ps, GradArgs ga, double* __restrict__ partial) {
-    const Piece c = piece_of<kCoarse>(ps);
-    const G* g = grad_of<G>(c, ga);
+// The piece's sum of g^2, in thread 0.  64 bits: the squares of finite floats do not overflow there.
+template <typename G> __device__ __forceinline__ double piece_squares(const Piece& c, const G* g) {
     double s = 0.0;
     if (g) {
         int i = threadIdx.x * 4;
@@ -53,21 +50,39 @@ __global__ __launch_bounds__(kBlock) void squares_kernel(Pieces ps, GradArgs ga,
         }
         for (; i < c.n; i += kBlock * 4) s = add_squares(s, to_float<4>(load_some<4, false, true>(g + i, c.n - i)));
     }
-    s = block_sum<kBlock>(s);
-    if (threadIdx.x == 0) partial[ps.first + dealt(blockIdx.x, gridDim.x)] = s;
+    return block_sum<kBlock>(s);
 }
 
-__device__ __forceinline__ float clip_coef(double norm, double max_norm) {
-    return norm > max_norm ? (float)(max_norm / norm) : 1.0f;
+// What becomes of the sums: entry t < count is tensor t, entry `count` all of them.
+struct NormsOut {
+    int count;
+    double scale, max_norm;
+    int each;
+    float *norms, *coefs;
+    int* nonfinite;
+
+    __device__ __forceinline__ void put(int t, double s) const {
+        const double norm = sqrt(s) * scale;
+        if (norms) norms[t] = (float)norm;
+        const float coef = norm > max_norm ? (float)(max_norm / norm) : 1.0f;
+        if (coefs && each && t < count) coefs[t] = coef;
+        if (coefs && !each && t == count) coefs[0] = coef;
+        if (nonfinite && t == count) *nonfinite = s <= 1.7976931348623157e308 ? 0 : 1;
+    }
+};
+
+template <typename G>
+__global__ __launch_bounds__(kBlock) void squares_kernel(Pieces ps, GradArgs ga, double* __restrict__ partial) {
+    const Piece c = piece_of<kCoarse>(ps);
+    const double s = piece_squares(c, grad_of<G>(c, ga));
+    if (threadIdx.x == 0) partial[ps.first + dealt(blockIdx.x, gridDim.x)] = s;
 }
 
 // Block t < count: tensor t's norm; block `count`: that of all, from all pieces' sums in a fixed order.
 __global__ __launch_bounds__(kBlock) void norms_kernel(const double* __restrict__ partial,
-                                                       const int* __restrict__ first_piece, int count, double scale,
-                                                       double max_norm, int each, float* __restrict__ norms,
-                                                       float* __restrict__ coefs, int* __restrict__ nonfinite) {
+                                                       const int* __restrict__ first_piece, NormsOut out) {
     const int t = blockIdx.x;
-    const int from = t < count ? first_piece[t] : 0, to = first_piece[t < count ? t + 1 : count];
+    const int from = t < out.count ? first_piece[t] : 0, to = first_piece[t < out.count ? t + 1 : out.count];
     double s = 0.0;
     int i = from + threadIdx.x;
     for (; i + 3 * kBlock < to; i += 4 * kBlock) {  // loads of one turn together
@@ -76,12 +91,36 @@ __global__ __launch_bounds__(kBlock) void norms_kernel(const double* __restrict_
     }
     for (; i < to; i += kBlock) s += partial[i];
     s = block_sum<kBlock>(s);
-    if (threadIdx.x != 0) return;
-    const double norm = sqrt(s) * scale;
-    if (norms) norms[t] = (float)norm;
-    if (coefs && each && t < count) coefs[t] = clip_coef(norm, max_norm);
-    if (coefs && !each && t == count) coefs[0] = clip_coef(norm, max_norm);
-    if (nonfinite && t == count) *nonfinite = s <= 1.7976931348623157e308 ? 0 : 1;
+    if (threadIdx.x == 0) out.put(t, s);
+}
+
+// Both in one launch, for sets of at most kBlock pieces and fewer tensors: the workgroup that finishes last
+// (`done` counts them, and is 0 again behind the launch) makes the norms.  No workgroup waits.  LeNet-5's ten
+// tensors: ... us a call against 8.0 us as two launches.
+template <typename G>
+__global__ __launch_bounds__(kBlock) void small_norms_kernel(Pieces ps, GradArgs ga, double* partial, unsigned* done,
+                                                             const int* __restrict__ first_piece, NormsOut out) {
+    __shared__ double sums[kBlock];
+    __shared__ unsigned last;
+    const Piece c = piece_of<kCoarse>(ps);
+    const double mine = piece_squares(c, grad_of<G>(c, ga));
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(partial + dealt(blockIdx.x, gridDim.x), mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    const int pieces = gridDim.x, i = threadIdx.x;
+    const double x = i < pieces ? __hip_atomic_load(partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    sums[i] = x;
+    if (i == 0) __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const double all = block_sum<kBlock>(x);  // (its barrier is the one that `sums` needs)
+    if (i < out.count) {
+        double s = 0.0;
+        for (int k = first_piece[i]; k < first_piece[i + 1]; ++k) s += sums[k];
+        out.put(i, s);
+    }
+    if (i == out.count) out.put(i, all);
 }
 
 template <typename G>
@@ -127,6 +166,8 @@ bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 
 }  // namespace
 
+static_assert(kBlock <= kGradsPerLaunch, "the gradients of a small set fit one launch");
+
 #define CX_NUM_DISPATCH(dt, CALL)                                                     \
     switch (dt) {                                                                     \
         case CX_F32: { using G = Num<CX_F32>::type; CALL; } break;                    \
@@ -136,14 +177,20 @@ bool aligned_to(const void* p, int bytes) { return reinterpret_cast<uintptr_t>(p
 
 int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale, double max_norm, int each,
                       float* d_norms, float* d_coefs, int* d_nonfinite) {
+    const NormsOut out = {t->count, std::fabs(scale), max_norm, each, d_norms, d_coefs, d_nonfinite};
+    const auto& cut = t->cut[kCoarse];
+    const bool small = cut.pieces > 0 && cut.pieces <= kBlock && t->count < kBlock;  // (one launch's gradients)
     int rc = for_grads(t, g, kCoarse, [&](const Pieces& ps, int n, const GradArgs& a) -> int {
-        CX_NUM_DISPATCH(g->type, (squares_kernel<G><<<n, kBlock, 0, h->stream>>>(ps, a, t->d_partial)));
+        if (small)
+            CX_NUM_DISPATCH(g->type, (small_norms_kernel<G><<<n, kBlock, 0, h->stream>>>(ps, a, t->d_partial, t->d_done,
+                                                                                         cut.d_first, out)))
+        else
+            CX_NUM_DISPATCH(g->type, (squares_kernel<G><<<n, kBlock, 0, h->stream>>>(ps, a, t->d_partial)))
         CX_HIP(hipGetLastError());
         return CX_OK;
     });
-    if (rc != CX_OK) return rc;
-    norms_kernel<<<t->count + 1, kBlock, 0, h->stream>>>(t->d_partial, t->cut[kCoarse].d_first, t->count, std::fabs(scale),
-                                                         max_norm, each, d_norms, d_coefs, d_nonfinite);
+    if (rc != CX_OK || small) return rc;
+    norms_kernel<<<t->count + 1, kBlock, 0, h->stream>>>(t->d_partial, cut.d_first, out);
     CX_HIP(hipGetLastError());
     return CX_OK;
 }
@@ -304,6 +351,8 @@ static int create_tensors(cx_tensors* out, cx_handle h, int count, const long lo
     }
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_partial), (t->cut[kCoarse].pieces + 1) * sizeof(double));
     if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_rates), 256);
+    const std::vector<unsigned> zero(1, 0u);
+    upload(&t->d_done, zero);
     const hipError_t waited = hipStreamSynchronize(h->stream);  // the host tables go away
     if (e == hipSuccess) e = waited;
     if (e != hipSuccess) return fail(CX_ERR_HIP, "cx_tensors_create: %s", hipGetErrorString(e));
@@ -331,6 +380,7 @@ int cx_tensors_destroy(cx_tensors t) {
     if (t->d_tensors) (void)hipFree(t->d_tensors);
     if (t->d_partial) (void)hipFree(t->d_partial);
     if (t->d_rates) (void)hipFree(t->d_rates);
+    if (t->d_done) (void)hipFree(t->d_done);
     delete t;
     return CX_OK;
 }
