@@ -26,9 +26,9 @@ struct alignas(16) Tensor {
 
 // The tensors are cut into pieces, one workgroup's work each; a tensor's last piece may be shorter.  `owner`
 // says which tensor a piece belongs to (4 bytes a piece, and the tensors' table stays in the caches).
-// kFine and kWide: what reads and writes, 4 or 8 elements a lane.  Pieces of one load per stream and lane: all workgroups in flight
-// then walk through each buffer as one narrow front.  fp32 step on 25.6 M elements: 122 us with 1024 elements
-// a piece, 128 with 2048, 141 with 4096, 151 with 16384 (loops over the piece), 159 with 65536.
+// kFine and kWide: what reads and writes, 4 or 8 elements a lane.  Pieces of one load per stream and lane: all
+// workgroups in flight then walk through each buffer as one narrow front.  fp32 step on 25.6 M elements: 122 us
+// with 1024 elements a piece, 128 with 2048, 141 with 4096, 151 with 16384 (loops over the piece), 159 with 65536.
 // kCoarse: the sums of squares, which want few partial sums.
 struct Pieces {
     const Tensor* tensors;

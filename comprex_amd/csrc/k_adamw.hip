@@ -240,8 +240,8 @@ __device__ __forceinline__ Codes v_codes(Vec<float, 8> v, float inverse) {
     Codes c = {};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const unsigned code = ((__float_as_uint(y[k]) + 0x80000u) >> 20) & 255u;   // (no finite value exceeds 255)
-        c.x[k / 4] |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * (k % 4));  // above 0: never 0
+        const unsigned code = min((__float_as_uint(y[k]) + 0x80000u) >> 20, 255u);  // above 255 only what is not finite
+        c.x[k / 4] |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * (k % 4));   // above 0: never 0
     }
     return c;
 }

@@ -52,14 +52,14 @@ def _addresses(tensors):
 
 class TensorSet:
     """The tensors of a training step (cx_tensors): how many elements each has, for `Handle.grad_norms`
-    and `Handle.pack`.  Made once per model and kept; belongs on one stream at a time, and a graph captured
-    with it needs it alive."""
+    and `Handle.pack`.  Made once per model and kept; belongs to its handle, whose stream everything a call takes
+    has to be ready on, and a graph captured with it needs it alive."""
 
     def __init__(self, handle, sizes):
         self._make(handle, [int(n) for n in sizes], None)
 
     def _make(self, handle, sizes, state):
-        self.lib, self.sizes = handle.lib, sizes
+        self.lib, self.handle, self.sizes = handle.lib, handle, sizes
         self._on(handle.device)
         self.total = sum(sizes)
         self._t = C.c_void_p()
@@ -130,6 +130,14 @@ class TensorSet:
         found.kept, found.of = each, self
         return found
 
+    def _new(self, n, dtype):
+        """A vector for the handle's stream to write: of that stream's memory where another one is current."""
+        # (torch.cuda.current_stream() makes an object each time: 2 us more)
+        if torch._C._cuda_getCurrentRawStream(self._where) == self.handle.stream.cuda_stream:
+            return torch.empty(n, dtype=dtype, device=self.device)
+        with torch.cuda.stream(self.handle.stream):
+            return torch.empty(n, dtype=dtype, device=self.device)
+
     def _coefs(self, coefs):
         if coefs is None:
             return None, 0
@@ -148,7 +156,7 @@ class TensorSet:
     def _vector(self, t, dtype, what):
         """A given vector of all elements, checked, or a new one."""
         if t is None:
-            return torch.empty(self.total, dtype=dtype, device=self.device)
+            return self._new(self.total, dtype)
         if t.dtype != dtype or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
             raise _invalid("%s is a contiguous vector of %s on %s", what, dtype, self.device)
         if t.numel() != self.total:
@@ -419,7 +427,7 @@ class Handle:
         for t, n, dt, what in ((norms, count + 1, torch.float32, "norms"), (coefs, count if each else 1, torch.float32, "coefs"),
                                (nonfinite, 1, torch.int32, "nonfinite")):
             if t is None:
-                t = torch.empty(n, dtype=dt, device=tensors.device)
+                t = tensors._new(n, dt)
             elif t.dtype != dt or t.device != tensors.device or t.numel() != n or not t.is_contiguous():
                 raise _invalid("%s: %d contiguous elements of %s on %s", what, n, dt, tensors.device)
             out.append(t)

@@ -100,6 +100,10 @@ class ComprexOptimizer(torch.optim.Optimizer):
             off += p.numel()
 
 
+#: the exchange counts in 32-bit integers
+_MOST_EXCHANGED = (1 << 31) - 1
+
+
 class _Part:
     """The parameters of one group that share a type and a width of the moments, and their AdamWSet."""
 
@@ -126,7 +130,11 @@ class ComprexAdamW(torch.optim.Optimizer):
     master_weights: bf16 and fp16 parameters get fp32 weights of which they are the rounded values.
     skip_nonfinite: a gradient with an infinity or NaN anywhere leaves its rank's moments and count as they are,
     and its weights too or, with several ranks, its part of the sum zero; decided on the device, where the steps
-    are counted then (a parameter without a gradient counts along with those it is stepped with).  Parameters are contiguous and on one GPU."""
+    are counted then (a parameter without a gradient counts along with those it is stepped with).
+
+    Parameters are contiguous and on one GPU.  The layout of the exchanged vector follows the parameters that require
+    a gradient: one that is frozen or released starts a new exchange, without what the old one held back.  A program
+    that captures its steps in a graph calls `Handle.grad_norms` and `Handle.adamw_step` itself."""
 
     def __init__(self, params, gaspi_env, learning_rate=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  clip_norm=None, state_bits=32, min_8bit_size=4096, master_weights=True, skip_nonfinite=False,
@@ -188,6 +196,9 @@ class ComprexAdamW(torch.optim.Optimizer):
         if self.master_weights and p.dtype != torch.float32:
             state["master"] = p.detach().to(torch.float32)
 
+    def _training(self):
+        return [p.requires_grad for group in self.param_groups for p in group["params"]]
+
     def _make_parts(self):
         parts = {}
         for k, group in enumerate(self.param_groups):
@@ -197,9 +208,11 @@ class ComprexAdamW(torch.optim.Optimizer):
                 self._check(p)
                 if "exp_avg" not in self.state[p]:
                     self._new_state(p)
-                key = (k, p.dtype, "exp_avg_scales" in self.state[p], "master" in self.state[p])
+                key = (k, p.dtype, "exp_avg_scales" in self.state[p], "master" in self.state[p],
+                       self.state[p]["step"] if self.skip_nonfinite else None)  # a part has one count on the device
                 parts.setdefault(key, _Part(group, [])).params.append(p)
         self._parts = list(parts.values())
+        self._trained = self._training()
 
     def _sync_counts(self):
         """The steps' counts where they live on the device, into the state (a saved state holds numbers)."""
@@ -265,6 +278,9 @@ class ComprexAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         ranks = self.gaspi_env.get_ranks()
+        if self._parts is not None and self._trained != self._training():  # parameters were frozen or released
+            self._sync_counts()
+            self._parts = None
         if self._parts is None:
             self._make_parts()
         if not self._parts:
@@ -277,8 +293,13 @@ class ComprexAdamW(torch.optim.Optimizer):
             for part, g, checked in zip(parts, lists, ready):
                 if checked is not None:
                     self._step_part(part, g, checked, coef, flag)
+                    torch.autograd.graph.increment_version([p for p, x in zip(part.params, g) if x is not None])
             return loss
         total = sum(part.set.total for part in parts)
+        if total > _MOST_EXCHANGED:
+            raise ValueError("an exchange takes at most %d elements, not %d" % (_MOST_EXCHANGED, total))
+        if total == 0:
+            return loss
         if self.blob is None or self.blob.numel() != total:
             self.blob = torch.empty(total, dtype=torch.float32, device=stream.device)
             self.allreduce = _make_allreduce(self.allreduce_type, self.gaspi_env, total, self.compression_ratio,
@@ -299,6 +320,7 @@ class ComprexAdamW(torch.optim.Optimizer):
         for part in parts:
             self.handle.adamw_apply(part.set, self.blob[at:at + part.set.total], part.group["lr"],
                                     part.group["weight_decay"], scale=1.0 / ranks)
+            torch.autograd.graph.increment_version(part.params)
             at += part.set.total
         return loss
 

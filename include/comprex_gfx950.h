@@ -320,7 +320,8 @@ typedef struct cx_tensors_s* cx_tensors;
  * (code 8 e + f stands for 2^(e-1) (1 + f/8), for f / 8 where e = 0), in units that give the block's
  * largest value V the code 255, scale V; a value above 0 never becomes code 0.  Both are rounded to
  * nearest.  A block whose M (or V) is below 2^-100 is stored as zeros with scale 0.  Elements that are not
- * finite count in no maximum: their exp_avg is stored as NaN and they leave their block's others alone.
+ * finite count in no maximum and leave their block's others alone: their exp_avg is stored as NaN, such an
+ * exp_avg_sq as the block's largest.
  * Bytes and scales that are zero stand for zero moments: how training begins. */
 enum { CX_STATE_BLOCK = 256 };
 typedef struct {

@@ -345,6 +345,33 @@ def test_tensors_that_move_and_streams_that_change():
     within(p, want.w, 5, 1e-2)
 
 
+def test_parameters_that_are_released_later():
+    env = pygpi.GaspiEnvironment()
+    a, b = parameter(np.ones(10, np.float32)), parameter(np.ones(10, np.float32))
+    b.requires_grad_(False)
+    opt = ComprexAdamW([a, b], env, learning_rate=0.5, weight_decay=0.0, skip_nonfinite=True)
+    a.grad = torch.ones_like(a)
+    opt.step()
+    b.requires_grad_(True)
+    b.grad = torch.ones_like(b)
+    versions = a._version, b._version
+    opt.step()
+    assert (a.detach().cpu() - 0.0).abs().max() < 1e-5      # two moves of 0.5
+    assert ((b.detach().cpu() - 0.5).abs() < 1e-5).all()    # one
+    assert a._version > versions[0] and b._version > versions[1]   # autograd sees the weights change
+
+
+def test_an_exchange_of_too_many_elements_is_refused(monkeypatch):
+    from comprex_amd import optimizer
+    monkeypatch.setattr(optimizer, "_MOST_EXCHANGED", 99)
+    env = pygpi.GaspiEnvironment()
+    env.set_rank(0, 2)
+    p = parameter(np.ones(100, np.float32))
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError):
+        ComprexAdamW([p], env).step()
+
+
 def test_refusals():
     env = pygpi.GaspiEnvironment()
     p = parameter(np.ones(10, np.float32))

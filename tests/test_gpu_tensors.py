@@ -151,6 +151,29 @@ def test_more_than_2_to_the_31_elements():
     assert all(float(out[at]) == 3 * x for at, x in marks.items())
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_on_more_than_2_to_the_31_elements(bits):
+    D = device_module()
+    sizes = [(1 << 31) + 5, 1000]
+    total, marks = sum(sizes), [0, (1 << 31) - 1, 1 << 31, (1 << 31) + 4, (1 << 31) + 5, sum(SIZE for SIZE in sizes) - 1]
+    g = torch.zeros(total, dtype=BF16, device="cuda")
+    g[torch.tensor(marks, device="cuda")] = 2.0
+    p = torch.zeros(total, dtype=BF16, device="cuda")
+    h = D.Handle()
+    split = lambda t: [t[:sizes[0]], t[sizes[0]:]]  # noqa: E731
+    if bits == 32:
+        m, v = torch.zeros(total, device="cuda"), torch.zeros(total, device="cuda")
+        s = D.AdamWSet(h, split(p), split(m), split(v))
+    else:
+        small = [D.AdamWSet.zeros8(x) for x in split(p)]
+        s = D.AdamWSet(h, split(p), *([x[k] for x in small] for k in (0, 1)), exp_avg_scales=[x[2] for x in small],
+                       exp_avg_sq_scales=[x[3] for x in small])
+    h.adamw_step(s, split(g), 1, 2.0 ** -7, weight_decay=0.0)   # a first step moves by lr
+    h.adamw_step(s, g, 2, 2.0 ** -7, weight_decay=0.0)
+    assert int(p.count_nonzero()) == len(marks)
+    assert all(abs(float(p[at]) + 2.0 ** -6) <= 2.0 ** -6 * 2.0 ** -7 for at in marks)
+
+
 # ---- AdamW -------------------------------------------------------------------------------------
 
 E4M3 = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
@@ -324,6 +347,55 @@ def test_adamw_step(sizes, param, grad, master, bits, offset):
         check_step(P, before, [f64(g) for g in grads], [x * scale for x in c], step, **hyper)
 
 
+@pytest.mark.parametrize("param,grad,master", [(F32, F32, False), (BF16, BF16, True), (F16, F16, False)], ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nothing_beside_the_tensors_is_written(bits, param, grad, master):
+    """Tensors between guards of a mark of their own: every kernel leaves them as they are."""
+    D = device_module()
+    sizes = [1, 2, 3, 5, 255, 257, 511, 513, 1023, 1025, 2047, 2049, 4100]
+    blocks = [-(-n // BLOCK) for n in sizes]
+    rooms = []
+
+    def guarded(ns, dtype):
+        """A buffer with 5 elements of guard before, between and behind parts of the given sizes."""
+        room = torch.full((sum(ns) + 5 * (len(ns) + 1),), 77, dtype=dtype, device="cuda")
+        inside = torch.zeros(room.numel(), dtype=torch.bool, device="cuda")
+        parts, at = [], 5
+        for n in ns:
+            room[at:at + n] = 0
+            inside[at:at + n] = True
+            parts.append(room[at:at + n])
+            at += n + 5
+        rooms.append((room, inside))
+        return parts
+
+    p, w = guarded(sizes, param), guarded(sizes, F32) if master else None
+    if bits == 32:
+        m, v, scales = guarded(sizes, F32), guarded(sizes, F32), []
+    else:
+        m, v = [x.view(torch.float8_e4m3fn) for x in guarded(sizes, torch.uint8)], guarded(sizes, torch.uint8)
+        scales = [guarded(blocks, F32), guarded(blocks, F32)]
+    h = D.Handle()
+    s = D.AdamWSet(h, p, m, v, w, *scales)
+    grads = [torch.ones(n, dtype=grad, device="cuda") for n in sizes]
+    flat, moves, norms, coefs = (guarded([n], F32)[0] for n in (sum(sizes), sum(sizes), len(sizes) + 1, len(sizes)))
+    h.grad_norms(s, grads, 1.0, each=True, norms=norms, coefs=coefs)
+    h.pack(s, grads, out=flat, coefs=coefs)
+    h.adamw_step(s, grads, 1, 0.5)
+    h.adamw_step(s, flat, 2, 0.5, moves=moves)
+    h.adamw_apply(s, moves, 0.5)
+    if bits == 8:
+        a, b = (guarded([sum(sizes)], BF16)[0] for _ in range(2))
+        c, d = (guarded([sum(sizes)], F32)[0] for _ in range(2))
+        h.adamw_states(s, BF16, a, b)
+        h.adamw_states(s, F32, c, d)
+        h.adamw_set_states(s, c, d)
+    h.synchronize()
+    for room, inside in rooms:
+        assert (room[~inside] == 77).all()
+        assert (room[inside] != 0).all()  # (and everything inside was)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_flat_gradient_is_the_list(bits):
     """The flat vector, as the exchange leaves it, against the same gradients one by one: the same bits."""
@@ -466,6 +538,21 @@ def test_nonfinite_elements_stay_alone(bits):
         assert torch.equal(v[fine], Q.v[0][fine])
 
 
+def test_8bit_second_moments_that_overflow_stay_the_largest():
+    """(1e20)^2 overflows fp32 though the gradient is finite: stored as the block's largest, not as something small."""
+    D = device_module()
+    p = torch.zeros(300, device="cuda")
+    state = D.AdamWSet.zeros8(p)
+    h = D.Handle()
+    s = D.AdamWSet(h, [p], [state[0]], [state[1]], exp_avg_scales=[state[2]], exp_avg_sq_scales=[state[3]])
+    g = torch.ones(300, device="cuda")
+    g[7] = 1e20
+    h.adamw_step(s, [g], 1, 1e-3)
+    m, v = h.adamw_states(s)
+    assert state[1][7] == 255 and float(v[7]) == float(state[3][0]) and torch.isfinite(v).all()
+    assert torch.equal(v[:7], v[8:15]) and torch.isfinite(p).all()
+
+
 def test_8bit_blocks_below_2_to_the_minus_100_are_zero():
     D = device_module()
     n = 3 * BLOCK + 5
@@ -554,6 +641,26 @@ def test_clip_pack_and_step_captured_and_replayed(bits):
         assert same(A.snapshot(), B.snapshot())
 
 
+def test_outputs_are_of_the_handles_stream():
+    """A handle on a stream of its own while another is current: what its calls allocate is that stream's memory."""
+    D = device_module()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        h = D.Handle()
+    s = D.TensorSet(h, [70001])
+    g = torch.ones(70001, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(20):
+        busy = torch.ones(70001, device="cuda")
+        for _ in range(20):
+            busy.mul_(1.0)
+        del busy  # its memory may be the current stream's next, while the stream is still at it
+        flat = h.pack(s, [g], scale=3.0)
+        norms = h.grad_norms(s, flat)[0]
+        side.synchronize()
+        assert (flat == 3).all() and abs(float(norms[0]) - 3 * math.sqrt(70001)) < 1e-3
+
+
 def test_refusals_on_the_device():
     D = device_module()
     h = D.Handle()
@@ -580,6 +687,9 @@ def test_refusals_on_the_device():
     refused(bad, h.adamw_step, s, [g], 1, 1e-3, eps=0.0)
     refused(bad, h.adamw_step, s, [g], 1, 1e-3, weight_decay=-1.0)
     refused(bad, h.adamw_step, s, [g], 1, 1e-3, scale=math.inf)
+    refused(bad, h.adamw_step, s, [g], 1, 1e-3, scale=1e39)         # not in fp32
+    refused(bad, h.adamw_step, s, [g], 1, 1e39)
+    refused(bad, h.pack, s, [g], scale=1e39)
     refused(size, h.adamw_step, s, [g], 1, 1e-3, coefs=torch.ones(2, device="cuda"))
     refused(bad, h.adamw_step, s, [g], 1, 1e-3, moves=torch.zeros(10, dtype=BF16, device="cuda"))
     refused(size, h.adamw_step, s, [g], 1, 1e-3, moves=torch.zeros(11, device="cuda"))
