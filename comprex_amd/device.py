@@ -130,6 +130,16 @@ class TensorSet:
         found.kept, found.of = each, self
         return found
 
+    def part_of(self, grads, start):
+        """The gradients of this set out of those that were checked as a list for a larger one, from its tensor `start`
+        on."""
+        sizes = grads.of.sizes[start:start + len(self.sizes)]
+        if grads.each is None or start < 0 or sizes != self.sizes or grads.of.device != self.device:
+            raise _invalid("these are not the gradients of this set's tensors", code=_lib.CX_ERR_SIZE_MISMATCH)
+        found = _lib.Grads(grads.type, grads.each + start * C.sizeof(C.c_void_p), None)
+        found.kept, found.of = grads.kept, self
+        return found
+
     def _new(self, n, dtype):
         """A vector for the handle's stream to write: of that stream's memory where another one is current."""
         # (torch.cuda.current_stream() makes an object each time: 2 us more)

@@ -17,10 +17,13 @@ average.  The schedules deliver each rank another vector and make up for it late
 such vectors would not and the ranks' weights would drift apart.  Clipping and the step run as a few launches
 over all tensors (`Handle.grad_norms`, `adamw_step`, `adamw_apply`), and nothing waits for the device.
 """
+import operator
+
 import torch
 
 from . import pygpi
-from .device import AdamWSet, Handle
+from ._lib import ComprexError
+from .device import AdamWSet, Handle, TensorSet
 
 _SCHEDULES = {
     "comprex_alltoone": pygpi.Comprex_AllToOneAllreduce,
@@ -104,6 +107,9 @@ class ComprexOptimizer(torch.optim.Optimizer):
 _MOST_EXCHANGED = (1 << 31) - 1
 
 
+_STATE = ("exp_avg", "exp_avg_sq", "master", "exp_avg_scales", "exp_avg_sq_scales")  # an AdamWSet's lists
+
+
 class _Part:
     """The parameters of one group that share a type and a width of the moments, and their AdamWSet."""
 
@@ -114,8 +120,26 @@ class _Part:
     def tensors(self, state):
         """params, exp_avg, exp_avg_sq, masters, scales of both: lists, or None."""
         states = [state[p] for p in self.params]
-        return [self.params] + [[s[k] for s in states] if k in states[0] else None
-                                for k in ("exp_avg", "exp_avg_sq", "master", "exp_avg_scales", "exp_avg_sq_scales")]
+        return [self.params] + [list(map(operator.itemgetter(k), states)) if k in states[0] else None for k in _STATE]
+
+
+class _Kind:
+    """The parts whose gradients share a type, and the set of all their gradients."""
+
+    def __init__(self, parts):
+        self.parts, self.set = parts, None
+        self.params = [p for part in parts for p in part.params]
+
+    def gradients(self):
+        """(the list, the same checked for the set); (list, None) where there is none at all."""
+        grads = list(map(operator.attrgetter("grad"), self.params))
+        try:
+            return grads, self.set.gradients(grads) if any(g is not None for g in grads) else None
+        except (ComprexError, RuntimeError):  # perhaps one of another layout
+            if any(g is not None and g.is_sparse for g in grads):
+                raise RuntimeError("ComprexAdamW takes dense gradients only") from None
+            grads = [None if g is None else g.contiguous() for g in grads]
+            return grads, self.set.gradients(grads)
 
 
 class ComprexAdamW(torch.optim.Optimizer):
@@ -156,7 +180,7 @@ class ComprexAdamW(torch.optim.Optimizer):
         self.master_weights, self.skip_nonfinite = master_weights, skip_nonfinite
         self.compression_ratio, self.allreduce_type, self.size_factor = compression_ratio, allreduce_type, size_factor
         self.handle = self.allreduce = self.blob = self._parts = None
-        self._exchange_stream = None
+        self._exchange_stream, self._order = None, []
 
     @staticmethod
     def _check(p):
@@ -211,8 +235,16 @@ class ComprexAdamW(torch.optim.Optimizer):
                 key = (k, p.dtype, "exp_avg_scales" in self.state[p], "master" in self.state[p],
                        self.state[p]["step"] if self.skip_nonfinite else None)  # a part has one count on the device
                 parts.setdefault(key, _Part(group, [])).params.append(p)
-        self._parts = list(parts.values())
+        self._parts = sorted(parts.values(), key=lambda part: str(part.params[0].dtype))  # a kind's follow one another
+        by_type = {}
+        for part in self._parts:
+            by_type.setdefault(part.params[0].dtype, []).append(part)
+        self._kinds = [_Kind(of_one) for of_one in by_type.values()]
         self._trained = self._training()
+        order = [p for kind in self._kinds for p in kind.params]
+        if len(order) != len(self._order) or not all(map(operator.is_, order, self._order)):
+            self.blob = None  # another layout: another exchange
+        self._order = order
 
     def _sync_counts(self):
         """The steps' counts where they live on the device, into the state (a saved state holds numbers)."""
@@ -232,12 +264,15 @@ class ComprexAdamW(torch.optim.Optimizer):
         if self.handle is None or self.handle.device != stream.device:
             with torch.cuda.device(stream.device):
                 self.handle = Handle(stream)
-            for part in self._parts:
-                part.set = None
+            for x in self._parts + self._kinds:
+                x.set = None
         self.handle.set_stream(stream)
+        for kind in self._kinds:
+            if kind.set is None:
+                kind.set = TensorSet(self.handle, [p.numel() for p in kind.params])
         for part in self._parts:
             lists = part.tensors(self.state)
-            now = [t.data_ptr() for x in lists if x is not None for t in x]
+            now = [list(map(torch.Tensor.data_ptr, x)) for x in lists if x is not None]
             if part.set is None or part.made_of != now:
                 part.set, part.made_of = AdamWSet(self.handle, *lists), now
                 if self.skip_nonfinite and part.count is None:
@@ -245,22 +280,13 @@ class ComprexAdamW(torch.optim.Optimizer):
                                             device=stream.device)
         return stream
 
-    def _grads(self, part):
-        grads = [p.grad for p in part.params]
-        for k, g in enumerate(grads):
-            if g is None:
-                continue
-            if g.is_sparse:
-                raise RuntimeError("ComprexAdamW takes dense gradients only")
-            if not g.is_contiguous():
-                grads[k] = g.contiguous()
-        return grads
-
-    def _clip(self, live):
+    def _clip(self, found):
         """(coefficient or None, non-finite flag or None) of all gradients together."""
-        if not live or (self.clip_norm is None and not self.skip_nonfinite):
+        found = [(kind, checked) for kind, _, checked in found if checked is not None]
+        if not found or (self.clip_norm is None and not self.skip_nonfinite):
             return None, None
-        found = [self.handle.grad_norms(part.set, g, self.clip_norm if len(live) == 1 else None) for part, g in live]
+        found = [self.handle.grad_norms(kind.set, checked, self.clip_norm if len(found) == 1 else None)
+                 for kind, checked in found]
         if len(found) == 1:
             norms, coef, flag = found[0]
         else:
@@ -286,31 +312,39 @@ class ComprexAdamW(torch.optim.Optimizer):
         if not self._parts:
             return loss
         stream = self._make_sets()
-        parts, lists = self._parts, [self._grads(part) for part in self._parts]
-        ready = [part.set.gradients(g) if any(x is not None for x in g) else None for part, g in zip(parts, lists)]
-        coef, flag = self._clip([(part, g) for part, g in zip(parts, ready) if g is not None])
+        found = [(kind, *kind.gradients()) for kind in self._kinds]
+        coef, flag = self._clip(found)
+        each = []  # (part, its gradients, the same checked or None)
+        for kind, grads, checked in found:
+            at = 0
+            for part in kind.parts:
+                own = grads[at:at + len(part.params)]
+                some = any(g is not None for g in own)
+                each.append((part, own, part.set.part_of(checked, at) if some else None))
+                at += len(own)
         if ranks == 1:
-            for part, g, checked in zip(parts, lists, ready):
+            for part, own, checked in each:
                 if checked is not None:
-                    self._step_part(part, g, checked, coef, flag)
-                    torch.autograd.graph.increment_version([p for p, x in zip(part.params, g) if x is not None])
+                    self._step_part(part, own, checked, coef, flag)
+                    torch.autograd.graph.increment_version([p for p, x in zip(part.params, own) if x is not None])
             return loss
+        parts = self._parts
         total = sum(part.set.total for part in parts)
         if total > _MOST_EXCHANGED:
             raise ValueError("an exchange takes at most %d elements, not %d" % (_MOST_EXCHANGED, total))
         if total == 0:
             return loss
-        if self.blob is None or self.blob.numel() != total:
+        if self.blob is None:
             self.blob = torch.empty(total, dtype=torch.float32, device=stream.device)
             self.allreduce = _make_allreduce(self.allreduce_type, self.gaspi_env, total, self.compression_ratio,
                                              self.size_factor)
         at = 0
-        for part, g, checked in zip(parts, lists, ready):
+        for part, own, checked in each:
             moves = self.blob[at:at + part.set.total]
-            if any(x is None for x in g):
+            if any(g is None for g in own):
                 moves.zero_()
             if checked is not None:
-                self._step_part(part, g, checked, coef, flag, moves)
+                self._step_part(part, own, checked, coef, flag, moves)
             at += part.set.total
         if stream.cuda_stream != (self._exchange_stream or 0):  # the exchange orders itself with this stream
             self.gaspi_env.set_user_stream(stream)

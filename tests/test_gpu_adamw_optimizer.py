@@ -361,6 +361,48 @@ def test_parameters_that_are_released_later():
     assert a._version > versions[0] and b._version > versions[1]   # autograd sees the weights change
 
 
+def test_gradients_of_two_types_are_clipped_together():
+    env = pygpi.GaspiEnvironment()
+    rng = np.random.default_rng(8)
+    x = [rng.standard_normal(n).astype(np.float32) for n in (5000, 300, 20)]
+    types = [torch.float32, BF16, torch.float32]
+    ps = [parameter(v, d) for v, d in zip(x, types)]
+    opt = ComprexAdamW(ps, env, learning_rate=1e-2, weight_decay=0.0, clip_norm=1.0, skip_nonfinite=True)
+    want = [Formula(f64(p)) for p in ps]
+    for step in range(3):
+        for p, v in zip(ps, x):
+            p.grad = torch.from_numpy(rng.standard_normal(v.size).astype(np.float32)).cuda().to(p.dtype)
+        gs = [f64(p.grad) for p in ps]
+        coef = min(1.0, 1.0 / math.sqrt(sum(float((g * g).sum()) for g in gs)))
+        opt.step()
+        for f, g in zip(want, gs):
+            f.step(g * coef, 1e-2, 0.0)
+    for p, f in zip(ps, want):
+        within(opt.state[p].get("master", p), f.w, 3, 1e-2)
+    before = [p.detach().clone() for p in ps]
+    ps[1].grad[4] = math.inf  # one type's, but all are skipped
+    opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, before))
+
+
+def test_another_layout_starts_another_exchange():
+    """Two parameters of one size, one frozen and then the other: what was held back for the first is not the second's."""
+    def program(env, rank):
+        a, b = parameter(np.zeros(100, np.float32)), parameter(np.zeros(100, np.float32))
+        b.requires_grad_(False)
+        opt = ComprexAdamW([a, b], env, learning_rate=1.0, weight_decay=0.0, compression_ratio=0.05, size_factor=3.0)
+        a.grad = torch.arange(1.0, 101.0, device="cuda")
+        opt.step()
+        a.requires_grad_(False)
+        b.requires_grad_(True)
+        env.barrier()
+        b.grad = torch.zeros(100, device="cuda")
+        opt.step()
+        assert b.count_nonzero() == 0
+
+    run_ranks(2, program)
+
+
 def test_an_exchange_of_too_many_elements_is_refused(monkeypatch):
     from comprex_amd import optimizer
     monkeypatch.setattr(optimizer, "_MOST_EXCHANGED", 99)

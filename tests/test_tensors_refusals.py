@@ -50,6 +50,19 @@ def test_gradients_are_checked():
     refused(bad, s.gradients, torch.zeros(16)[::2])
 
 
+def test_a_part_of_the_gradients_is_the_list_from_there_on():
+    s, part = host_set([3, 0, 5, 5]), host_set([0, 5])
+    grads = [torch.zeros(3), torch.zeros(0), None, torch.ones(5)]
+    whole = s.gradients(grads)
+    own = part.part_of(whole, 1)
+    assert own.of is part and list((C.c_void_p * 2).from_address(own.each)) == [None, None]
+    assert part.gradients(own) is own
+    assert list((C.c_void_p * 1).from_address(host_set([5]).part_of(whole, 3).each)) == [grads[3].data_ptr()]
+    for n, start in (([0, 5], 0), ([0, 5], 2), ([5, 5, 5], 2), ([5], 4), ([5], -1)):
+        refused(_lib.CX_ERR_SIZE_MISMATCH, host_set(n).part_of, whole, start)
+    refused(_lib.CX_ERR_SIZE_MISMATCH, host_set([8]).part_of, host_set([8]).gradients(torch.zeros(8)), 0)  # a flat one
+
+
 def test_vectors_coefficients_and_single_values_are_checked():
     s = host_set([3, 5])
     bad, size = _lib.CX_ERR_INVALID, _lib.CX_ERR_SIZE_MISMATCH
