@@ -153,6 +153,8 @@ int coarse_step(long long total) {
 constexpr long long kMostElements = 1ll << 33;
 constexpr int kMostTensors = 1 << 20;
 
+constexpr int kLine = 32;  // fp32 elements of 128 bytes
+
 struct Span {
     uintptr_t from, to;
 };
@@ -326,10 +328,12 @@ static int create_tensors(cx_tensors* out, cx_handle h, int count, const long lo
                 x.v_scale = state->exp_avg_sq_scales[k];
             }
         }
+        if (state && state->state_bits == 32) x.lead = (int)(reinterpret_cast<uintptr_t>(x.m) / 4 % kLine);
         for (int w = 0; w < kDivisions; ++w) {
             x.first[w] = (int)owner[w].size();
             t->cut[w].first.push_back(x.first[w]);
-            owner[w].insert(owner[w].end(), (size_t)((sizes[k] + t->cut[w].step - 1) / t->cut[w].step), k);
+            const long long n = sizes[k] > 0 && w == kFine ? sizes[k] + x.lead : sizes[k];
+            owner[w].insert(owner[w].end(), (size_t)((n + t->cut[w].step - 1) / t->cut[w].step), k);
         }
         t->sizes.push_back(sizes[k]);
         t->flat.push_back(flat);
