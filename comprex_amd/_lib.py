@@ -2,6 +2,8 @@
 the cx_* prototypes of include/comprex_gfx950.h.  There is no fallback: a missing
 library is an error."""
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import subprocess
 
@@ -117,6 +119,23 @@ def lib():
         fn.argtypes = args
     _lib = L
     return L
+
+
+_lists = None
+
+
+def tensor_lists():
+    """The module that looks at lists of torch tensors (comprex_amd/csrc/torch)."""
+    global _lists
+    if _lists is None:
+        path = os.path.join(_HERE, "lib", "_tensor_lists.so")
+        if not os.path.exists(path):
+            raise ImportError("%s is missing: build it with `make -C comprex_amd/csrc` "
+                              "(or __graft_entry__.build())" % path)
+        loader = importlib.machinery.ExtensionFileLoader("_tensor_lists", path)
+        _lists = importlib.util.module_from_spec(importlib.util.spec_from_loader("_tensor_lists", loader))
+        loader.exec_module(_lists)
+    return _lists
 
 
 def check(rc):

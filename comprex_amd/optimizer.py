@@ -114,13 +114,14 @@ class _Part:
     """The parameters of one group that share a type and a width of the moments, and their AdamWSet."""
 
     def __init__(self, group, params):
-        self.group, self.params = group, params
-        self.set = self.made_of = self.count = None
+        self.group, self.params, self.states = group, params, []
+        self.set = self.count = None
 
     def tensors(self, state):
         """params, exp_avg, exp_avg_sq, masters, scales of both: lists, or None."""
-        states = [state[p] for p in self.params]
-        return [self.params] + [list(map(operator.itemgetter(k), states)) if k in states[0] else None for k in _STATE]
+        self.states = list(map(state.__getitem__, self.params))
+        return [self.params] + [list(map(operator.itemgetter(k), self.states)) if k in self.states[0] else None
+                                for k in _STATE]
 
 
 class _Kind:
@@ -272,9 +273,8 @@ class ComprexAdamW(torch.optim.Optimizer):
                 kind.set = TensorSet(self.handle, [p.numel() for p in kind.params])
         for part in self._parts:
             lists = part.tensors(self.state)
-            now = [list(map(torch.Tensor.data_ptr, x)) for x in lists if x is not None]
-            if part.set is None or part.made_of != now:
-                part.set, part.made_of = AdamWSet(self.handle, *lists), now
+            if part.set is None or not part.set.made_of(lists):
+                part.set = AdamWSet(self.handle, *lists)
                 if self.skip_nonfinite and part.count is None:
                     part.count = torch.full((1,), self.state[part.params[0]]["step"], dtype=torch.int32,
                                             device=stream.device)
@@ -366,11 +366,11 @@ class ComprexAdamW(torch.optim.Optimizer):
         if part.count is not None:
             self.handle.adamw_step(part.set, checked, part.count, group["lr"], **how)
             return
-        states = [self.state[p] for p in part.params]
-        for s, g in zip(states, grads):
+        counts = set()
+        for s, g in zip(part.states, grads):
             if g is not None:
-                s["step"] += 1
-        counts = sorted({s["step"] for s, g in zip(states, grads) if g is not None})
-        for n in counts:  # one, unless some parameter went without a gradient before
-            these = checked if len(counts) == 1 else [g if s["step"] == n else None for s, g in zip(states, grads)]
+                s["step"] = n = s["step"] + 1
+                counts.add(n)
+        for n in sorted(counts):  # one, unless some parameter went without a gradient before
+            these = checked if len(counts) == 1 else [g if s["step"] == n else None for s, g in zip(part.states, grads)]
             self.handle.adamw_step(part.set, these, n, group["lr"], **how)

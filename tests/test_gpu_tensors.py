@@ -661,6 +661,28 @@ def test_outputs_are_of_the_handles_stream():
         assert (flat == 3).all() and abs(float(norms[0]) - 3 * math.sqrt(70001)) < 1e-3
 
 
+def test_lists_out_of_the_ordinary():
+    """What the native look at a list leaves to Python: taken where it is sound, refused by name where it is not."""
+    D = device_module()
+    h = D.Handle()
+    s = D.TensorSet(h, [6, 4])
+    a, b = torch.arange(6.0, device="cuda"), torch.ones(4, device="cuda")
+    want = torch.cat([a, b])
+    assert torch.equal(h.pack(s, [a, b]), want)
+    assert torch.equal(h.pack(s, (a, b)), want)
+    assert torch.equal(h.pack(s, [a.view(2, 3), torch.nn.Parameter(b)]), want)
+    half = h.pack(s, [a.half(), None])
+    assert torch.equal(half, torch.cat([a, torch.zeros(4, device="cuda")]))
+    for code, grads in ((_lib.CX_ERR_SIZE_MISMATCH, [a]), (_lib.CX_ERR_SIZE_MISMATCH, [b, a]),
+                        (_lib.CX_ERR_INVALID, [a, b.cpu()]), (_lib.CX_ERR_INVALID, [a, b.double()]),
+                        (_lib.CX_ERR_INVALID, [a, b.half()]), (_lib.CX_ERR_INVALID, [a.double(), b.double()]),
+                        (_lib.CX_ERR_INVALID, [a, torch.ones(8, device="cuda")[::2]]),
+                        (_lib.CX_ERR_INVALID, [a, torch.ones(4, device="meta")])):
+        with pytest.raises(ComprexError) as e:
+            h.pack(s, grads)
+        assert e.value.code == code
+
+
 def test_refusals_on_the_device():
     D = device_module()
     h = D.Handle()

@@ -63,6 +63,28 @@ def test_a_part_of_the_gradients_is_the_list_from_there_on():
     refused(_lib.CX_ERR_SIZE_MISMATCH, host_set([8]).part_of, host_set([8]).gradients(torch.zeros(8)), 0)  # a flat one
 
 
+def test_the_native_look_at_lists_answers_the_ordinary_case_only():
+    """Host tensors, things that are no tensors and lists of another length are left to the checks in Python."""
+    L = _lib.tensor_lists()
+    sizes, out = (C.c_longlong * 2)(3, 4), (C.c_uint64 * 2)(7, 7)
+    look = lambda x, n=2: L.addresses(x, n, C.addressof(sizes), C.addressof(out), 0)  # noqa: E731
+    assert look([None, None]) == _lib.CX_F32 and list(out) == [0, 0]
+    for x in ([torch.zeros(3), None], [None, 5], [None], [None] * 3, (None, None), "ab", [None, torch.zeros(4, device="meta")],
+              [torch.zeros(3).to_sparse(), None]):
+        assert look(x) == -1
+    with pytest.raises(TypeError):
+        L.addresses([], 0)
+    with pytest.raises(TypeError):
+        L.unmoved([], 0)
+    with pytest.raises((TypeError, OverflowError)):
+        L.addresses([], 0, -1, 0, 0)
+    a, b = torch.zeros(3), torch.zeros(4)
+    at = (C.c_uint64 * 2)(a.data_ptr(), b.data_ptr())
+    assert L.unmoved([a, b], 2, C.addressof(at))
+    for x in ([b, a], [a, b.clone()], [a], [a, None], (a, b), [a, 5]):
+        assert not L.unmoved(x, 2, C.addressof(at))
+
+
 def test_vectors_coefficients_and_single_values_are_checked():
     s = host_set([3, 5])
     bad, size = _lib.CX_ERR_INVALID, _lib.CX_ERR_SIZE_MISMATCH
