@@ -181,6 +181,7 @@ struct cx_tensors_s {
     int param_type = 0, state_bits = 0;
     bool masters = false;
     // device
+    void* memory = nullptr;                 // holds all of the following
     cx::Tensor* d_tensors = nullptr;
     double* d_partial = nullptr;            // per coarse piece: sum of the gradient's squares
     unsigned* d_done = nullptr;             // workgroups of small_norms_kernel that are through; 0 between launches

@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <exception>
 #include <memory>
 
@@ -339,28 +340,44 @@ static int create_tensors(cx_tensors* out, cx_handle h, int count, const long lo
         t->flat.push_back(flat);
         flat += sizes[k];
     }
-    hipError_t e = hipSuccess;
-    auto upload = [&](auto** to, const auto& from) {
-        if (e != hipSuccess) return;
-        const size_t bytes = from.size() * sizeof(from[0]);
-        e = hipMalloc(reinterpret_cast<void**>(to), bytes ? bytes : 1);
-        if (e == hipSuccess && bytes) e = hipMemcpyAsync(*to, from.data(), bytes, hipMemcpyHostToDevice, h->stream);
+    // one allocation: the tables, uploaded at once, and the scratch behind them
+    std::vector<char> tables;
+    size_t bytes = 0;
+    auto place = [&](const void* from, size_t n) {  // where it will lie
+        const size_t at = bytes;
+        bytes = at + (n + 255) / 256 * 256;
+        if (from) {
+            tables.resize(bytes);
+            if (n) std::memcpy(tables.data() + at, from, n);
+        }
+        return at;
     };
-    upload(&t->d_tensors, tensors);
+    const size_t at_tensors = place(tensors.data(), tensors.size() * sizeof(Tensor));
+    size_t at_owner[kDivisions], at_first[kDivisions];
     for (int w = 0; w < kDivisions; ++w) {
         auto& cut = t->cut[w];
         cut.pieces = (int)owner[w].size();
         cut.first.push_back(cut.pieces);
-        upload(&cut.d_owner, owner[w]);
-        upload(&cut.d_first, cut.first);
+        at_owner[w] = place(owner[w].data(), owner[w].size() * sizeof(int));
+        at_first[w] = place(cut.first.data(), cut.first.size() * sizeof(int));
     }
-    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_partial), (t->cut[kCoarse].pieces + 1) * sizeof(double));
-    if (e == hipSuccess) e = hipMalloc(reinterpret_cast<void**>(&t->d_rates), 256);
-    const std::vector<unsigned> zero(1, 0u);
-    upload(&t->d_done, zero);
-    const hipError_t waited = hipStreamSynchronize(h->stream);  // the host tables go away
-    if (e == hipSuccess) e = waited;
+    const unsigned zero = 0;
+    const size_t at_done = place(&zero, sizeof zero);
+    const size_t at_rates = place(nullptr, 256);
+    const size_t at_partial = place(nullptr, t->cut[kCoarse].pieces * sizeof(double));
+    hipError_t e = hipMalloc(&t->memory, bytes);
+    if (e == hipSuccess) e = hipMemcpyAsync(t->memory, tables.data(), tables.size(), hipMemcpyHostToDevice, h->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(h->stream);  // the host's tables go away
     if (e != hipSuccess) return fail(CX_ERR_HIP, "cx_tensors_create: %s", hipGetErrorString(e));
+    char* base = static_cast<char*>(t->memory);
+    t->d_tensors = reinterpret_cast<Tensor*>(base + at_tensors);
+    for (int w = 0; w < kDivisions; ++w) {
+        t->cut[w].d_owner = reinterpret_cast<int*>(base + at_owner[w]);
+        t->cut[w].d_first = reinterpret_cast<int*>(base + at_first[w]);
+    }
+    t->d_done = reinterpret_cast<unsigned*>(base + at_done);
+    t->d_rates = reinterpret_cast<float*>(base + at_rates);
+    t->d_partial = reinterpret_cast<double*>(base + at_partial);
     *out = made.release();
     return CX_OK;
 }
@@ -378,14 +395,7 @@ int cx_tensors_create(cx_tensors* out, cx_handle h, int count, const long long* 
 int cx_tensors_destroy(cx_tensors t) {
     if (!t) return CX_OK;
     DeviceScope on(t->device);
-    for (auto& cut : t->cut) {  // freeing waits for the device
-        if (cut.d_owner) (void)hipFree(cut.d_owner);
-        if (cut.d_first) (void)hipFree(cut.d_first);
-    }
-    if (t->d_tensors) (void)hipFree(t->d_tensors);
-    if (t->d_partial) (void)hipFree(t->d_partial);
-    if (t->d_rates) (void)hipFree(t->d_rates);
-    if (t->d_done) (void)hipFree(t->d_done);
+    if (t->memory) (void)hipFree(t->memory);  // waits for the device
     delete t;
     return CX_OK;
 }
