@@ -81,18 +81,19 @@ __global__ __launch_bounds__(kBlock) void squares_kernel(Pieces ps, GradArgs ga,
 }
 
 // Block t < count: tensor t's norm; block `count`: that of all, from all pieces' sums in a fixed order.
-__global__ __launch_bounds__(kBlock) void norms_kernel(const double* __restrict__ partial,
+constexpr int kNormsBlock = 1024;
+__global__ __launch_bounds__(kNormsBlock) void norms_kernel(const double* __restrict__ partial,
                                                        const int* __restrict__ first_piece, NormsOut out) {
     const int t = blockIdx.x;
     const int from = t < out.count ? first_piece[t] : 0, to = first_piece[t < out.count ? t + 1 : out.count];
     double s = 0.0;
     int i = from + threadIdx.x;
-    for (; i + 3 * kBlock < to; i += 4 * kBlock) {  // loads of one turn together
-        const double a = partial[i], b = partial[i + kBlock], c = partial[i + 2 * kBlock], d = partial[i + 3 * kBlock];
+    for (; i + 3 * kNormsBlock < to; i += 4 * kNormsBlock) {  // loads of one turn together
+        const double a = partial[i], b = partial[i + kNormsBlock], c = partial[i + 2 * kNormsBlock], d = partial[i + 3 * kNormsBlock];
         s += (a + b) + (c + d);
     }
-    for (; i < to; i += kBlock) s += partial[i];
-    s = block_sum<kBlock>(s);
+    for (; i < to; i += kNormsBlock) s += partial[i];
+    s = block_sum<kNormsBlock>(s);
     if (threadIdx.x == 0) out.put(t, s);
 }
 
@@ -194,7 +195,7 @@ int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale
         return CX_OK;
     });
     if (rc != CX_OK || small) return rc;
-    norms_kernel<<<t->count + 1, kBlock, 0, h->stream>>>(t->d_partial, cut.d_first, out);
+    norms_kernel<<<t->count + 1, kNormsBlock, 0, h->stream>>>(t->d_partial, cut.d_first, out);
     CX_HIP(hipGetLastError());
     return CX_OK;
 }
