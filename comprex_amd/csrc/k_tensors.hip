@@ -238,6 +238,21 @@ int check_grads(cx_tensors t, const cx_grads* g, const char* who) {
     return CX_OK;
 }
 
+// A flat output lies apart from the gradients, or an element on the gradient it is made of.
+int check_apart(cx_tensors t, const cx_grads* grads, const float* out, const char* who) {
+    const char *lo = reinterpret_cast<const char*>(out), *hi = lo + t->total * 4;
+    const int bytes = element_bytes(grads->type);
+    for (int k = 0; k < t->count; ++k) {
+        if (t->sizes[k] == 0) continue;  // (of an empty set neither form of the gradients need be there)
+        const char* g = grads->flat ? static_cast<const char*>(grads->flat) + t->flat[k] * bytes
+                                    : static_cast<const char*>(grads->each[k]);
+        if (!g || g >= hi || g + t->sizes[k] * bytes <= lo) continue;
+        if (grads->type != CX_F32 || g != lo + t->flat[k] * 4)
+            return fail(CX_ERR_INVALID, "%s: the output overlaps gradient %d", who, k);
+    }
+    return CX_OK;
+}
+
 int check_coefs(cx_tensors t, const float* d_coefs, int n_coefs, const char* who) {
     if (n_coefs != 0 && n_coefs != 1 && n_coefs != t->count)
         return fail(CX_ERR_SIZE_MISMATCH, "%s: %d coefficients for %d tensors", who, n_coefs, t->count);
@@ -421,16 +436,8 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
     if (rc != CX_OK) return rc;
     if (!std::isfinite((float)scale)) return fail(CX_ERR_INVALID, "cx_pack: scale must be finite in fp32");
     if ((!out && t->total > 0) || !aligned_to(out, 4)) return fail(CX_ERR_INVALID, "cx_pack: null or misaligned output");
-    const char *lo = reinterpret_cast<const char*>(out), *hi = lo + t->total * 4;
-    const int bytes = element_bytes(grads->type);
-    for (int k = 0; k < t->count; ++k) {
-        if (t->sizes[k] == 0) continue;  // (of an empty set neither form of the gradients need be there)
-        const char* g = grads->flat ? static_cast<const char*>(grads->flat) + t->flat[k] * bytes
-                                    : static_cast<const char*>(grads->each[k]);
-        if (!g || g >= hi || g + t->sizes[k] * bytes <= lo) continue;
-        if (grads->type != CX_F32 || g != lo + t->flat[k] * 4)
-            return fail(CX_ERR_INVALID, "cx_pack: the output overlaps gradient %d", k);
-    }
+    rc = check_apart(t, grads, out, "cx_pack");
+    if (rc != CX_OK) return rc;
     DeviceScope on(t->device);
     CX_HIP(on.error);
     return launch_pack(h, t, grads, n_coefs ? d_coefs : nullptr, n_coefs, (float)scale, d_skip, out);
@@ -453,6 +460,7 @@ int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_ada
         return fail(CX_ERR_INVALID, "cx_adamw_step: the weight decay must be finite and not negative");
     if (!std::isfinite((float)a->scale)) return fail(CX_ERR_INVALID, "cx_adamw_step: scale must be finite");
     if (!aligned_to(a->d_moves, 4)) return fail(CX_ERR_INVALID, "cx_adamw_step: misaligned moves");
+    if (a->d_moves && (rc = check_apart(t, grads, a->d_moves, "cx_adamw_step")) != CX_OK) return rc;
     if (!a->d_step && a->step < 1) return fail(CX_ERR_INVALID, "cx_adamw_step: steps count from 1");
     DeviceScope on(t->device);
     CX_HIP(on.error);

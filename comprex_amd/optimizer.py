@@ -105,8 +105,6 @@ class ComprexOptimizer(torch.optim.Optimizer):
 
 #: the exchange counts in 32-bit integers
 _MOST_EXCHANGED = (1 << 31) - 1
-
-
 _STATE = ("exp_avg", "exp_avg_sq", "master", "exp_avg_scales", "exp_avg_sq_scales")  # an AdamWSet's lists
 
 
@@ -207,6 +205,7 @@ class ComprexAdamW(torch.optim.Optimizer):
             if i in state_dict["state"]:
                 self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
                                  for k, v in state_dict["state"][i].items()}
+                self.state[p]["step"] = int(self.state[p]["step"])  # (torch's own optimizers save a tensor)
         self._parts = None
 
     def _new_state(self, p):

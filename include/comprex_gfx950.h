@@ -380,7 +380,7 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
  *
  * d_moves != NULL: only the moments take the step, and what w would lose to it, lr / (1 - beta1^step) * m / (...),
  * goes to this flat fp32 vector (the tensors back to back; *d_skip != 0: zeros; a tensor without a gradient: left
- * as it is) for the exchange to sum.  Ranks whose vectors differ for a while, as the compressed schedules leave
+ * as it is) for the exchange to sum; it may be the flat fp32 gradient itself, as cx_pack's output.  Ranks whose vectors differ for a while, as the compressed schedules leave
  * them, end up with the same weights that way (sums are delivered late, never lost), as they do with the momentum
  * terms of keras/comprex_optimizer.py:97-133; moments of their own of differing sums would drift apart.
  * cx_adamw_apply is the other half: w = w (1 - lr weight_decay) - scale * moves, for every tensor of the set. */

@@ -361,6 +361,31 @@ def test_parameters_that_are_released_later():
     assert a._version > versions[0] and b._version > versions[1]   # autograd sees the weights change
 
 
+def test_a_state_of_torchs_own_adamw_is_taken():
+    """fp32 moments and counts of torch.optim.AdamW: the same formula goes on from them."""
+    env = pygpi.GaspiEnvironment()
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal(3000).astype(np.float32)
+    p, q = parameter(x), parameter(x)
+    theirs = torch.optim.AdamW([p], lr=1e-2, weight_decay=0.1)
+    ours = ComprexAdamW([q], env, learning_rate=1e-2, weight_decay=0.1)
+    want = Formula(f64(p))
+    for step in range(6):
+        g = rng.standard_normal(3000).astype(np.float32)
+        if step == 3:
+            with torch.no_grad():
+                q.copy_(p)
+            saved = theirs.state_dict()
+            saved["param_groups"] = ours.state_dict()["param_groups"]
+            ours.load_state_dict(saved)
+        opt, w = (theirs, p) if step < 3 else (ours, q)
+        w.grad = torch.from_numpy(g).cuda()
+        opt.step()
+        want.step(g.astype(np.float64), 1e-2, 0.1)
+    assert ours.state[q]["step"] == 6
+    within(q, want.w, 6, 1e-2)
+
+
 def test_gradients_of_two_types_are_clipped_together():
     env = pygpi.GaspiEnvironment()
     rng = np.random.default_rng(8)

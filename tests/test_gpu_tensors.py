@@ -470,6 +470,12 @@ def test_adamw_moves_and_apply_are_the_step(param, grad, master, bits, offset):
         assert same(w, (B.p, B.w))  # the weights wait for the other half
         B.h.adamw_apply(B.set, moves, 1e-2, 0.2)
         assert same(A.snapshot(), B.snapshot())
+    # in place of the flat gradient
+    flat = torch.cat([g.float() for g in grads])
+    C, E = (Params(10, sizes, param, bits, master, offset) for _ in range(2))
+    C.h.adamw_step(C.set, flat, 1, 1e-2, scale=scale, moves=moves)
+    E.h.adamw_step(E.set, flat, 1, 1e-2, scale=scale, moves=flat)
+    assert torch.equal(moves, flat) and same(C.snapshot(), E.snapshot())
     # without a gradient: its part of the moves is left
     moves.fill_(5.0)
     grads[2] = None
@@ -728,6 +734,7 @@ def test_refusals_on_the_device():
     refused(bad, h.pack, plain, room[5:], out=room[:10])
     half = torch.zeros(20, dtype=BF16, device="cuda")
     refused(bad, h.pack, plain, [half[:10]], out=half.view(torch.float32))
+    refused(bad, h.adamw_step, s, [room[5:]], 1, 1e-3, moves=room[:10])
     # a tensor twice, and buffers that overlap
     refused(bad, D.AdamWSet, h, [p, p], [z(), z()], [z(), z()])
     m = z()
