@@ -5,6 +5,9 @@ Tolerances count roundings: u = 2^-24 of a value for one rounding to fp32 (const
 rates that were rounded on the host count as one), half a step of the type for the last rounding of a
 16-bit parameter or an 8-bit state."""
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -645,6 +648,15 @@ def test_clip_pack_and_step_captured_and_replayed(bits):
         assert count.item() == k
         assert all(torch.equal(a, b) for a, b in zip(kept, (flat, norms, coefs)))
         assert same(A.snapshot(), B.snapshot())
+
+
+def test_from_plain_c():
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "tensors_test")
+    assert os.path.exists(exe), "build tests/cpp first (make -C tests/cpp, or __graft_entry__.build())"
+    print("running", exe, file=sys.stderr, flush=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    sys.stderr.write(r.stdout[-3000:] + r.stderr[-2000:])
+    assert r.returncode == 0 and "+++ PASSED +++" in r.stdout, r.stdout[-2000:]
 
 
 def test_outputs_are_of_the_handles_stream():
