@@ -173,6 +173,7 @@ struct cx_tensors_s {
     struct Division {
         int step = 0;                       // elements of a piece
         int pieces = 0;
+        int longest = 0;                    // most pieces of one tensor
         std::vector<int> first;             // count + 1
         int* d_owner = nullptr;
         int* d_first = nullptr;             // `first` on the device

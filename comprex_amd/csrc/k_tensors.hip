@@ -97,9 +97,12 @@ __global__ __launch_bounds__(kNormsBlock) void norms_kernel(const double* __rest
     if (threadIdx.x == 0) out.put(t, s);
 }
 
-// Both in one launch, for sets of at most kBlock pieces and fewer tensors: the workgroup that finishes last
-// (`done` counts them, and is 0 again behind the launch) makes the norms.  No workgroup waits.  LeNet-5's ten
-// tensors: 4.7 us a call against 8.0 us as two launches.
+// Both in one launch, for sets of at most kBlock pieces and fewer tensors, the longest of kSmallTensor pieces: the
+// workgroup that finishes last (`done` counts them, and is 0 again behind the launch) makes the norms.  No workgroup
+// waits.  One launch against two, us a call: 61 706 elements in 10 tensors 5.9 and 9.1, 2^18 in 50 (100 pieces) 6.3 and
+// 9.1, 638 976 in 200 (200 pieces) 8.6 and 9.4, 2^18 in one (64 pieces, which one thread adds) 7.6 and 9.1; beyond the
+// limits 2^20 in one tensor 17.7 and 9.0.
+constexpr int kSmallTensor = 64;
 template <typename G>
 __global__ __launch_bounds__(kBlock) void small_norms_kernel(Pieces ps, GradArgs ga, double* partial, unsigned* done,
                                                              const int* __restrict__ first_piece, NormsOut out) {
@@ -184,7 +187,8 @@ int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale
                       float* d_norms, float* d_coefs, int* d_nonfinite) {
     const NormsOut out = {t->count, std::fabs(scale), max_norm, each, d_norms, d_coefs, d_nonfinite};
     const auto& cut = t->cut[kCoarse];
-    const bool small = cut.pieces > 0 && cut.pieces <= kBlock && t->count < kBlock;  // (one launch's gradients)
+    const bool small = cut.pieces > 0 && cut.pieces <= kBlock && t->count < kBlock &&  // (one launch's gradients)
+                       cut.longest <= kSmallTensor;
     int rc = for_grads(t, g, kCoarse, [&](const Pieces& ps, int n, const GradArgs& a) -> int {
         if (small)
             CX_NUM_DISPATCH(g->type, (small_norms_kernel<G><<<n, kBlock, 0, h->stream>>>(ps, a, t->d_partial, t->d_done,
@@ -350,7 +354,9 @@ static int create_tensors(cx_tensors* out, cx_handle h, int count, const long lo
             x.first[w] = (int)owner[w].size();
             t->cut[w].first.push_back(x.first[w]);
             const long long n = sizes[k] > 0 && w == kFine ? sizes[k] + x.lead : sizes[k];
-            owner[w].insert(owner[w].end(), (size_t)((n + t->cut[w].step - 1) / t->cut[w].step), k);
+            const int pieces = (int)((n + t->cut[w].step - 1) / t->cut[w].step);
+            owner[w].insert(owner[w].end(), pieces, k);
+            t->cut[w].longest = std::max(t->cut[w].longest, pieces);
         }
         t->sizes.push_back(sizes[k]);
         t->flat.push_back(flat);

@@ -60,7 +60,7 @@ def half_step(dtype, x):
 @pytest.mark.parametrize("offset", [0, 1])
 @pytest.mark.parametrize("each", [False, True])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("sizes", SIZES + [[1200003, 5, 70001]], ids=str)  # the last: two launches for the norms
+@pytest.mark.parametrize("sizes", SIZES + [[262144], [262145], [1200003, 5, 70001]], ids=str)  # both sides of one launch
 def test_norms_and_pack(sizes, dtype, each, offset):
     D = device_module()
     rng = np.random.default_rng(len(sizes) + offset)
