@@ -8,12 +8,14 @@
 
 namespace {
 
-// cx_dtype of parameters and gradients (include/comprex_gfx950.h)
+// cx_dtype of parameters and gradients (include/comprex_gfx950.h), and the types of 8-bit moments
 int type_code(at::ScalarType t) {
     switch (t) {
         case at::kFloat: return 0;
         case at::kBFloat16: return 3;
         case at::kHalf: return 4;
+        case at::kFloat8_e4m3fn: return 100;
+        case at::kByte: return 101;
         default: return -1;
     }
 }
@@ -41,7 +43,8 @@ int addresses_of(PyObject* list, const int64_t* sizes, uint64_t* out, int64_t de
 }
 
 // addresses(tensors, count, sizes, out, device): `sizes` the address of the `count` int64 element counts they have to
-// have, `out` that of as many uint64 (0 for None), `device` the GPU they have to be on.  Their cx_dtype, or -1.
+// have, `out` that of as many uint64 (0 for None), `device` the GPU they have to be on.  Their type (type_code; 0 of
+// nothing but None), or -1.
 PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 5) {
         PyErr_SetString(PyExc_TypeError, "addresses(tensors, count, sizes, out, device)");
@@ -84,7 +87,7 @@ PyObject* unmoved(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef methods[] = {{"addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(addresses)), METH_FASTCALL,
-                          "addresses(tensors, count, sizes, out, device) -> cx_dtype or -1"},
+                          "addresses(tensors, count, sizes, out, device) -> type or -1"},
                          {"unmoved", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(unmoved)), METH_FASTCALL,
                           "unmoved(tensors, count, at) -> bool"},
                          {nullptr, nullptr, 0, nullptr}};

@@ -41,9 +41,8 @@ def _invalid(text, *args, code=_lib.CX_ERR_INVALID):
     return ComprexError(code, text % args)
 
 
-def _addresses(tensors):
-    """Host array of the tensors' addresses (None: no tensor)."""
-    return (C.c_void_p * len(tensors))(*[None if t is None else t.data_ptr() for t in tensors])
+# what the native look at a list calls its tensors' types
+_TYPE_CODES = {**_NUM, torch.float8_e4m3fn: 100, torch.uint8: 101}
 
 
 class TensorSet:
@@ -104,7 +103,7 @@ class TensorSet:
         n, each = len(grads), array.array("Q", bytes(8 * len(grads)))
         at = each.buffer_info()[0]
         code = self._addresses(grads, n, C.addressof(self._sizes), at, self._where) if self._addresses else -1
-        if code < 0:  # something is out of the ordinary
+        if not 0 <= code <= CX_F16:  # something is out of the ordinary
             code = self._examine(grads, each)
         found = _lib.Grads(code, at, None)
         found.kept, found.of = each, self
@@ -202,24 +201,32 @@ class AdamWSet(TensorSet):
         wanted = [("params", dtype, sizes), ("exp_avg", torch.float8_e4m3fn if small else f32, sizes),
                   ("exp_avg_sq", torch.uint8 if small else f32, sizes), ("masters", f32, sizes),
                   ("exp_avg_scales", f32, blocks), ("exp_avg_sq_scales", f32, blocks)]
+        self.kept, self._at = lists, []
         for got, (name, dt, ns) in zip(lists, wanted):
             if got is None:
+                self._at.append(None)
                 continue
             if len(got) != len(sizes):
                 raise _invalid("%d %s for %d parameters", len(got), name, len(sizes), code=_lib.CX_ERR_SIZE_MISMATCH)
-            for t, n in zip(got, ns):
-                if t.numel() != n:
-                    raise _invalid("%s has %d elements where %d belong", name, t.numel(), n,
-                                   code=_lib.CX_ERR_SIZE_MISMATCH)
-                if t.dtype != dt or t.device != handle.device or not t.is_contiguous():
-                    raise _invalid("%s are contiguous tensors of %s on %s", name, dt, handle.device)
-        self.kept = lists
-        self._at = [None if x is None else array.array("Q", [t.data_ptr() for t in x]) for x in lists]
+            at, counts = array.array("Q", bytes(8 * len(got))), array.array("q", ns)
+            if _lib.tensor_lists().addresses(got, len(got), counts.buffer_info()[0], at.buffer_info()[0],
+                                             -1 if handle.device.index is None else handle.device.index) != _TYPE_CODES[dt]:
+                self._examine_list(got, ns, name, dt, handle.device, at)
+            self._at.append(at)
         self.state_bits = 8 if small else 32
-        arrays = [None if x is None else _addresses(x) for x in lists]
-        at = [None if a is None else C.cast(a, C.c_void_p) for a in arrays]
+        at = [None if a is None else a.buffer_info()[0] for a in self._at]
         self._make(handle, sizes, C.byref(_lib.AdamwState(_NUM[dtype], self.state_bits, at[0], at[3], at[1], at[2], at[4],
                                                           at[5])))
+
+    @staticmethod
+    def _examine_list(tensors, sizes, name, dtype, device, at):
+        """Raises what is wrong with a list, or takes its addresses."""
+        for k, (t, n) in enumerate(zip(tensors, sizes)):
+            if t.numel() != n:
+                raise _invalid("%s has %d elements where %d belong", name, t.numel(), n, code=_lib.CX_ERR_SIZE_MISMATCH)
+            if t.dtype != dtype or t.device != device or not t.is_contiguous():
+                raise _invalid("%s are contiguous tensors of %s on %s", name, dtype, device)
+            at[k] = t.data_ptr()
 
     def made_of(self, lists):
         """Whether the set was made of these tensors where they are now: lists in __init__'s order."""

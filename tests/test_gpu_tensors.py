@@ -751,6 +751,14 @@ def test_refusals_on_the_device():
     refused(bad, D.AdamWSet, h, [p, p], [z(), z()], [z(), z()])
     m = z()
     refused(bad, D.AdamWSet, h, [p], [m], [m])
+    refused(bad, D.AdamWSet, h, [p], [None], [z()])
+    refused(bad, D.AdamWSet, h, [p], [z().cpu()], [z()])
+    refused(bad, D.AdamWSet, h, [p], [z().double()], [z()])
+    refused(bad, D.AdamWSet, h, [p], [torch.zeros(20, device="cuda")[::2]], [z()])
+    refused(size, D.AdamWSet, h, [p], [torch.zeros(11, device="cuda")], [z()])
+    small = D.AdamWSet.zeros8(p)
+    refused(bad, D.AdamWSet, h, [p], [small[0]], [small[0]], None, [small[2]], [small[3]])   # codes of the wrong kind
+    refused(bad, D.AdamWSet, h, [p], [small[1]], [small[1].clone()], None, [small[2]], [small[3]])
     both = torch.zeros(15, device="cuda")
     refused(bad, D.AdamWSet, h, [p, z()], [both[:10], both[5:]], [z(), z()])
     before = p.clone()
