@@ -260,6 +260,7 @@ def same(a, b):
 
 def check_step(P, before, g, factor, step, lr, b1, b2, eps, wd, tensors=None):
     """P's tensors against one step from `before`, with gradients g (64 bits) times factor[k]."""
+    now = P.now()
     for k in range(len(P.sizes)) if tensors is None else tensors:
         w, m, v = before[k]
         x = g[k] * factor[k]
@@ -281,7 +282,7 @@ def check_step(P, before, g, factor, step, lr, b1, b2, eps, wd, tensors=None):
         em_move = rate * em / below + np.abs(move) * (eb / (below - eb) + 5.01 * U)
         w1 = w - lr * wd * w - move
         ew = em_move + U * (3 * np.abs(lr * wd * w) + 2 * np.abs(move) + 1.01 * np.abs(w1))
-        got_w, got_m, got_v = P.now()[k]
+        got_w, got_m, got_v = now[k]
         if P.w is not None:
             assert (np.abs(got_w - w1) <= ew).all(), (k, np.abs(got_w - w1).max())
         p = f64(P.p[k])
@@ -424,6 +425,48 @@ def test_adamw_leaves_tensors_without_a_gradient(bits):
     assert same(even(now), even(was))
     check_step(P, before, [None if g is None else f64(g) for g in grads], [1.0] * 501, 7, 1e-2, 0.9, 0.999, 1e-8, 0.3,
                tensors=range(1, 501, 20))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_coefficient_per_tensor_beyond_one_launch(bits):
+    """A thousand tensors, three launches' addresses: each with the coefficient of its own, and packed with it too."""
+    sizes = [1 + k % 300 for k in range(1000)]
+    P = Params(12, sizes, F32, bits, False, 0)
+    before = P.now()
+    grads, _ = P.gradients(BF16, 0)
+    coefs = torch.as_tensor(P.rng.uniform(0.2, 1.0, 1000), dtype=F32).cuda()
+    flat = P.h.pack(P.set, grads, coefs=coefs)
+    assert torch.equal(flat, torch.cat([g.float() * c for g, c in zip(grads, coefs)]))
+    P.h.adamw_step(P.set, grads, 5, 1e-3, coefs=coefs)
+    check_step(P, before, [f64(g) for g in grads], list(f64(coefs)), 5, 1e-3, 0.9, 0.999, 1e-8, 0.01)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_on_scalars_and_on_one_gradient_given_twice(bits):
+    sizes = [1, 300, 300, 1]
+    A, B = (Params(13, sizes, F32, bits, False, 0) for _ in range(2))
+    g = torch.randn(300, device="cuda")
+    x, y = torch.tensor(0.25, device="cuda"), torch.tensor([[-2.0]], device="cuda")
+    A.h.adamw_step(A.set, [x, g, g, y], 1, 1e-3)
+    B.h.adamw_step(B.set, [x.view(1).clone(), g.clone(), g.clone(), y.view(1).clone()], 1, 1e-3)
+    assert same(A.snapshot(), B.snapshot())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_host_count_with_a_flag_or_a_rate_on_the_device(bits):
+    """Each of the device's values by itself: the flag with a host count, the rate with a host count."""
+    sizes = [3000, 7]
+    A, B = (Params(14, sizes, F32, bits, False, 0) for _ in range(2))
+    rate = torch.full((1,), 2e-3, device="cuda")
+    skip = torch.ones(1, dtype=torch.int32, device="cuda")
+    for step in (1, 2, 30):
+        grads, _ = A.gradients(F32, 0)
+        was = B.snapshot()
+        B.h.adamw_step(B.set, grads, step, 2e-3, skip=skip)
+        assert same(was, B.snapshot())
+        A.h.adamw_step(A.set, grads, step, float(rate))
+        B.h.adamw_step(B.set, grads, step, rate, skip=torch.zeros_like(skip))
+        assert same(A.snapshot(), B.snapshot())
 
 
 @pytest.mark.parametrize("bits", [32, 8])
