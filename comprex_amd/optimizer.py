@@ -156,8 +156,10 @@ class ComprexAdamW(torch.optim.Optimizer):
     are counted then (a parameter without a gradient counts along with those it is stepped with).
 
     Parameters are contiguous and on one GPU.  The layout of the exchanged vector follows the parameters that require
-    a gradient: one that is frozen or released starts a new exchange, without what the old one held back.  A program
-    that captures its steps in a graph calls `Handle.grad_norms` and `Handle.adamw_step` itself."""
+    a gradient: one that is frozen or released starts a new exchange, without what the old one held back.  With several
+    ranks a step leaves the stream it ran on as the environment's user stream of its thread: a program with exchanges of
+    its own sets theirs before them.  A program that captures its steps in a graph calls `Handle.grad_norms` and
+    `Handle.adamw_step` itself."""
 
     def __init__(self, params, gaspi_env, learning_rate=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
                  clip_norm=None, state_bits=32, min_8bit_size=4096, master_weights=True, skip_nonfinite=False,
@@ -179,7 +181,7 @@ class ComprexAdamW(torch.optim.Optimizer):
         self.master_weights, self.skip_nonfinite = master_weights, skip_nonfinite
         self.compression_ratio, self.allreduce_type, self.size_factor = compression_ratio, allreduce_type, size_factor
         self.handle = self.allreduce = self.blob = self._parts = None
-        self._exchange_stream, self._order = None, []
+        self._order = []
 
     @staticmethod
     def _check(p):
@@ -345,9 +347,8 @@ class ComprexAdamW(torch.optim.Optimizer):
             if checked is not None:
                 self._step_part(part, own, checked, coef, flag, moves)
             at += part.set.total
-        if stream.cuda_stream != (self._exchange_stream or 0):  # the exchange orders itself with this stream
-            self.gaspi_env.set_user_stream(stream)
-            self._exchange_stream = stream.cuda_stream
+        # the exchange orders itself with this stream; the setting belongs to the thread, and others change it too
+        self.gaspi_env.set_user_stream(stream)
         self.allreduce.apply(self.blob)  # in place, on the device
         at = 0
         for part in parts:
