@@ -17,6 +17,7 @@ average.  The schedules deliver each rank another vector and make up for it late
 such vectors would not and the ranks' weights would drift apart.  Clipping and the step run as a few launches
 over all tensors (`Handle.grad_norms`, `adamw_step`, `adamw_apply`), and nothing waits for the device.
 """
+import itertools
 import operator
 
 import torch
@@ -109,17 +110,24 @@ _STATE = ("exp_avg", "exp_avg_sq", "master", "exp_avg_scales", "exp_avg_sq_scale
 
 
 class _Part:
-    """The parameters of one group that share a type and a width of the moments, and their AdamWSet."""
+    """Parameters of one group that share a type and a width of the moments, and their AdamWSet.  `counts`: where the
+    steps are counted on the device, a count for each number that the parameters begin with, and whose it is."""
 
     def __init__(self, group, params):
         self.group, self.params, self.states = group, params, []
-        self.set = self.count = None
+        self.set, self.counts = None, []
 
     def tensors(self, state):
         """params, exp_avg, exp_avg_sq, masters, scales of both: lists, or None."""
         self.states = list(map(state.__getitem__, self.params))
         return [self.params] + [list(map(operator.itemgetter(k), self.states)) if k in self.states[0] else None
                                 for k in _STATE]
+
+    def count_on(self, device):
+        members = {}
+        for k, s in enumerate(self.states):
+            members.setdefault(s["step"], set()).add(k)
+        self.counts = [(torch.full((1,), n, dtype=torch.int32, device=device), ks) for n, ks in members.items()]
 
 
 class _Kind:
@@ -210,10 +218,14 @@ class ComprexAdamW(torch.optim.Optimizer):
                 self.state[p]["step"] = int(self.state[p]["step"])  # (torch's own optimizers save a tensor)
         self._parts = None
 
+    def _small(self, p):
+        """Whether a parameter's moments begin in 8 bits."""
+        return self.state_bits == 8 and p.numel() >= self.min_8bit_size
+
     def _new_state(self, p):
         state = self.state[p]
         state["step"] = 0
-        if self.state_bits == 8 and p.numel() >= self.min_8bit_size:
+        if self._small(p):
             (state["exp_avg"], state["exp_avg_sq"], state["exp_avg_scales"],
              state["exp_avg_sq_scales"]) = AdamWSet.zeros8(p)
         else:
@@ -226,7 +238,10 @@ class ComprexAdamW(torch.optim.Optimizer):
         return [p.requires_grad for group in self.param_groups for p in group["params"]]
 
     def _make_parts(self):
-        parts = {}
+        """The parts, in the order of the exchanged vector.  That follows from the groups, the types and the optimizer's
+        settings, which all ranks share; where a rank's states differ from them (another width was loaded, steps were
+        skipped), a part is divided where it stands."""
+        alike = {}
         for k, group in enumerate(self.param_groups):
             for p in group["params"]:
                 if not p.requires_grad:
@@ -234,10 +249,14 @@ class ComprexAdamW(torch.optim.Optimizer):
                 self._check(p)
                 if "exp_avg" not in self.state[p]:
                     self._new_state(p)
-                key = (k, p.dtype, "exp_avg_scales" in self.state[p], "master" in self.state[p],
-                       self.state[p]["step"] if self.skip_nonfinite else None)  # a part has one count on the device
-                parts.setdefault(key, _Part(group, [])).params.append(p)
-        self._parts = sorted(parts.values(), key=lambda part: str(part.params[0].dtype))  # a kind's follow one another
+                alike.setdefault((str(p.dtype), k, self._small(p)), []).append(p)
+
+        def form(p):
+            return "exp_avg_scales" in self.state[p], "master" in self.state[p]
+
+        self._parts = [_Part(self.param_groups[k], list(params))
+                       for (_, k, _), those in sorted(alike.items(), key=lambda x: x[0][0])  # a kind's follow one another
+                       for _, params in itertools.groupby(those, form)]
         by_type = {}
         for part in self._parts:
             by_type.setdefault(part.params[0].dtype, []).append(part)
@@ -251,10 +270,10 @@ class ComprexAdamW(torch.optim.Optimizer):
     def _sync_counts(self):
         """The steps' counts where they live on the device, into the state (a saved state holds numbers)."""
         for part in getattr(self, "_parts", None) or ():
-            if part.count is not None:
-                n = int(part.count)
-                for p in part.params:
-                    self.state[p]["step"] = n
+            for count, members in part.counts:
+                n = int(count)
+                for k in members:
+                    self.state[part.params[k]]["step"] = n
 
     def state_dict(self):
         self._sync_counts()
@@ -276,9 +295,8 @@ class ComprexAdamW(torch.optim.Optimizer):
             lists = part.tensors(self.state)
             if part.set is None or not part.set.made_of(lists):
                 part.set = AdamWSet(self.handle, *lists)
-                if self.skip_nonfinite and part.count is None:
-                    part.count = torch.full((1,), self.state[part.params[0]]["step"], dtype=torch.int32,
-                                            device=stream.device)
+                if self.skip_nonfinite and not part.counts:
+                    part.count_on(stream.device)
         return stream
 
     def _clip(self, found):
@@ -363,8 +381,14 @@ class ComprexAdamW(torch.optim.Optimizer):
         group = part.group
         how = dict(betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], coefs=coef, skip=flag,
                    moves=moves)
-        if part.count is not None:
-            self.handle.adamw_step(part.set, checked, part.count, group["lr"], **how)
+        for count, members in part.counts:
+            these = checked
+            if len(part.counts) > 1:
+                these = [g if k in members else None for k, g in enumerate(grads)]
+                if all(g is None for g in these):
+                    continue
+            self.handle.adamw_step(part.set, these, count, group["lr"], **how)
+        if part.counts:
             return
         counts = set()
         for s, g in zip(part.states, grads):

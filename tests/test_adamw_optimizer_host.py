@@ -233,3 +233,82 @@ def test_a_step_from_another_thread_sets_that_threads_stream():
         assert not errors, errors
 
     run_ranks(2, program)
+
+
+def recorded(opt):
+    """Where each parameter's moves lay in the last exchanged vector, by the values that were put there."""
+    return opt.allreduce.log[-1].tolist()
+
+
+@pytest.mark.parametrize("restore", [False, True])
+def test_the_vectors_layout_does_not_depend_on_a_ranks_counts(restore):
+    """Rank 1 skips a step (a NaN in its gradient) while the middle one of three parameters is frozen; then it is
+    released, or a state saved before is loaded, which groups the parameters by their counts anew.  Every weight gets
+    the average of its own moves."""
+    def program(env, rank):
+        ps = [parameter(n) for n in (3, 4, 5)]
+        ps[1].requires_grad_(False)
+        opt = ComprexAdamW(ps, env, weight_decay=0.0, skip_nonfinite=True)
+        for k in (0, 2):
+            give([ps[k]], float(k + 1))
+        if rank == 1:
+            ps[0].grad[1] = float("nan")
+        opt.step()
+        counts = [s["step"] for s in opt.state_dict()["state"].values()]
+        assert counts == ([1, 1], [0, 0])[rank]
+        ps[1].requires_grad_(True)
+        want = [1.0] * 3 + [2.0] * 4 + [3.0] * 5
+        for again in range(2):
+            for k in range(3):
+                give([ps[k]], float(k + 1))
+            opt.step()
+            assert recorded(opt) == want
+            if restore:
+                opt.load_state_dict(opt.state_dict())
+        assert [s["step"] for s in opt.state_dict()["state"].values()] == ([3, 3, 2], [2, 2, 2])[rank]
+        # the first step moved by half of rank 0's, the others by everything
+        for k, first in ((0, 0.5), (1, 0.0), (2, 0.5)):
+            assert torch.equal(ps[k].detach(), torch.full_like(ps[k], -(k + 1) * (2 + first)))
+
+    run_ranks(2, program)
+
+
+def test_the_vectors_layout_does_not_depend_on_what_a_rank_loaded():
+    """Rank 1 goes on from a state in 32 bits, rank 0 starts anew in 8: parameters lie in the same places."""
+    def program(env, rank):
+        ps = [parameter(n) for n in (300, 20, 400)]
+        opt = ComprexAdamW(ps, env, weight_decay=0.0, state_bits=8, min_8bit_size=100)
+        if rank == 1:
+            saved = ComprexAdamW(ps, Env(), weight_decay=0.0)
+            give(ps, 0.0)
+            saved.step()
+            opt.load_state_dict(saved.state_dict())
+        for k, p in enumerate(ps):
+            give([p], float(k + 1))
+        opt.step()
+        assert ("exp_avg_scales" in opt.state[ps[0]]) == (rank == 0)
+        for k, p in enumerate(ps):
+            assert torch.equal(p.detach(), torch.full_like(p, -(k + 1.0)))
+
+    run_ranks(2, program)
+
+
+def test_counts_of_a_part_on_the_device():
+    """One rank, counts on the device: parameters of different counts in one part each advance their own, those without
+    a gradient none of their own count's go along."""
+    env = Env()
+    ps = [parameter(3) for _ in range(4)]
+    for p in ps[2:]:
+        p.requires_grad_(False)
+    opt = ComprexAdamW(ps, env, weight_decay=0.0, skip_nonfinite=True)
+    give(ps[:2], 1.0)
+    opt.step()
+    for p in ps[2:]:
+        p.requires_grad_(True)
+    give(ps, 1.0)
+    ps[3].grad = None
+    opt.step()
+    ps[0].grad = ps[1].grad = None
+    opt.step()
+    assert [s["step"] for s in opt.state_dict()["state"].values()] == [2, 2, 2, 2]
+    assert [float(p[0]) for p in ps] == [-2, -2, -2, 0]
