@@ -164,7 +164,8 @@ class ComprexAdamW(torch.optim.Optimizer):
     are counted then (a parameter without a gradient counts along with those it is stepped with).
 
     Parameters are contiguous and on one GPU.  The layout of the exchanged vector follows the parameters that require
-    a gradient: one that is frozen or released starts a new exchange, without what the old one held back.  With several
+    a gradient: one that is frozen or released starts a new exchange, without what the old one held back (`flush`
+    delivers that before).  `load_state_dict`, which every rank calls, drops what is held back.  With several
     ranks a step leaves the stream it ran on as the environment's user stream of its thread: a program with exchanges of
     its own sets theirs before them.  A program that captures its steps in a graph calls `Handle.grad_norms` and
     `Handle.adamw_step` itself."""
@@ -217,6 +218,8 @@ class ComprexAdamW(torch.optim.Optimizer):
                                  for k, v in state_dict["state"][i].items()}
                 self.state[p]["step"] = int(self.state[p]["step"])  # (torch's own optimizers save a tensor)
         self._parts = None
+        if self.allreduce is not None:
+            self.allreduce.reset()  # what it held back are moves of the run that ends here
 
     def _small(self, p):
         """Whether a parameter's moments begin in 8 bits."""
@@ -264,7 +267,7 @@ class ComprexAdamW(torch.optim.Optimizer):
         self._trained = self._training()
         order = [p for kind in self._kinds for p in kind.params]
         if len(order) != len(self._order) or not all(map(operator.is_, order, self._order)):
-            self.blob = None  # another layout: another exchange
+            self.blob = self.allreduce = None  # another layout: another exchange
         self._order = order
 
     def _sync_counts(self):
@@ -278,6 +281,15 @@ class ComprexAdamW(torch.optim.Optimizer):
     def state_dict(self):
         self._sync_counts()
         return super().state_dict()
+
+    def _ready(self):
+        """The parts and their sets as the parameters are now; the current stream, or None if nothing is trained."""
+        if self._parts is not None and self._trained != self._training():  # parameters were frozen or released
+            self._sync_counts()
+            self._parts = None
+        if self._parts is None:
+            self._make_parts()
+        return self._make_sets() if self._parts else None
 
     def _make_sets(self):
         """The parts' sets, made anew where a tensor has moved (a state that was replaced, a model that was)."""
@@ -323,14 +335,9 @@ class ComprexAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         ranks = self.gaspi_env.get_ranks()
-        if self._parts is not None and self._trained != self._training():  # parameters were frozen or released
-            self._sync_counts()
-            self._parts = None
-        if self._parts is None:
-            self._make_parts()
-        if not self._parts:
+        stream = self._ready()
+        if stream is None:
             return loss
-        stream = self._make_sets()
         found = [(kind, *kind.gradients()) for kind in self._kinds]
         coef, flag = self._clip(found)
         each = []  # (part, its gradients, the same checked or None)
@@ -347,8 +354,7 @@ class ComprexAdamW(torch.optim.Optimizer):
                     self._step_part(part, own, checked, coef, flag)
                     torch.autograd.graph.increment_version([p for p, x in zip(part.params, own) if x is not None])
             return loss
-        parts = self._parts
-        total = sum(part.set.total for part in parts)
+        total = sum(part.set.total for part in self._parts)
         if total > _MOST_EXCHANGED:
             raise ValueError("an exchange takes at most %d elements, not %d" % (_MOST_EXCHANGED, total))
         if total == 0:
@@ -368,13 +374,30 @@ class ComprexAdamW(torch.optim.Optimizer):
         # the exchange orders itself with this stream; the setting belongs to the thread, and others change it too
         self.gaspi_env.set_user_stream(stream)
         self.allreduce.apply(self.blob)  # in place, on the device
+        self._apply(ranks)
+        return loss
+
+    def _apply(self, ranks, decay=True):
+        """What came back from the exchange, into the weights."""
         at = 0
-        for part in parts:
-            self.handle.adamw_apply(part.set, self.blob[at:at + part.set.total], part.group["lr"],
-                                    part.group["weight_decay"], scale=1.0 / ranks)
+        for part in self._parts:
+            self.handle.adamw_apply(part.set, self.blob[at:at + part.set.total], part.group["lr"] if decay else 0.0,
+                                    part.group["weight_decay"] if decay else 0.0, scale=1.0 / ranks)
             torch.autograd.graph.increment_version(part.params)
             at += part.set.total
-        return loss
+
+    @torch.no_grad()
+    def flush(self):
+        """Takes the moves that the exchange still holds back into the weights, where and as far as its schedule's flush
+        delivers them (the big ring: everywhere; all-to-one: on the chief).  They are in no saved state: every rank
+        calls this before it saves one, and before its parameters are frozen or released."""
+        stream = self._ready()
+        if stream is None or self.allreduce is None:
+            return
+        self.blob.zero_()
+        self.gaspi_env.set_user_stream(stream)
+        self.allreduce.flush(self.blob)
+        self._apply(self.gaspi_env.get_ranks(), decay=False)
 
     def _step_part(self, part, grads, checked, coef, flag, moves=None):
         """The step of a part's parameters that have a gradient (`checked`: the same, ready for the set)."""

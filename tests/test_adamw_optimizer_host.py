@@ -312,3 +312,71 @@ def test_counts_of_a_part_on_the_device():
     opt.step()
     assert [s["step"] for s in opt.state_dict()["state"].values()] == [2, 2, 2, 2]
     assert [float(p[0]) for p in ps] == [-2, -2, -2, 0]
+
+
+class Holding(Exchange):
+    """Delivers a rank its own vector and holds back what the others sent until it is flushed."""
+
+    def __init__(self, *args):
+        super().__init__(*args)
+        self.held = torch.zeros(self.size)
+
+    def swap(self, blob):
+        self.env.given[here.rank] = blob.clone()
+        self.env.meet.wait()
+        others = sum(self.env.given) - blob
+        self.env.meet.wait()
+        return others
+
+    def apply(self, blob):
+        self.joined()
+        self.held += self.swap(blob)
+
+    def flush(self, blob):
+        self.joined()
+        self.swap(blob)
+        blob += self.held
+        self.reset()
+
+    def reset(self):
+        super().reset()
+        self.held.zero_()
+
+
+def test_a_restored_state_gets_nothing_of_the_run_it_replaces(monkeypatch):
+    monkeypatch.setattr(optimizer, "_make_allreduce", Holding)
+
+    def program(env, rank):
+        ps = [parameter(3), parameter(4)]
+        opt = ComprexAdamW(ps, env, weight_decay=0.0)
+        opt.flush()  # nothing to flush yet
+        give(ps, 2.0 * (rank + 1))
+        opt.step()
+        assert float(ps[0][0]) == -(rank + 1)    # a half of its own; the other's is held back
+        opt.flush()
+        assert all((p == -3.0).all() for p in ps)
+        saved, kept = opt.state_dict(), [p.detach().clone() for p in ps]
+        give(ps, 64.0)
+        opt.step()                             # of a run that is given up
+        opt.load_state_dict(saved)
+        with torch.no_grad():
+            for p, k in zip(ps, kept):
+                p.copy_(k)
+        give(ps, 0.0)
+        opt.step()
+        opt.flush()
+        assert all((p == -3.0).all() for p in ps)
+        versions = [p._version for p in ps]
+        opt.flush()
+        assert all(p._version > v for p, v in zip(ps, versions)) and opt.blob.count_nonzero() == 0
+
+    run_ranks(2, program)
+
+
+def test_a_flush_by_one_rank_alone_changes_nothing():
+    ps = [parameter(3, 1.0)]
+    opt = ComprexAdamW(ps, Env(), weight_decay=0.5)
+    give(ps, 0.0)
+    opt.step()
+    opt.flush()
+    assert (ps[0] == 1.0).all() and opt.allreduce is None
