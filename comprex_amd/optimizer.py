@@ -360,6 +360,8 @@ class ComprexAdamW(torch.optim.Optimizer):
         if total == 0:
             return loss
         if self.blob is None:
+            # a channel grows for a larger vector: what an exchange before this one sent has to be read by then
+            self.gaspi_env.barrier()
             self.blob = torch.empty(total, dtype=torch.float32, device=stream.device)
             self.allreduce = _make_allreduce(self.allreduce_type, self.gaspi_env, total, self.compression_ratio,
                                              self.size_factor)

@@ -27,6 +27,7 @@ class Here(threading.local):
     rank = 0
     stream = Stream(0)
     user_stream = None
+    met = False
 
 
 here = Here()
@@ -380,3 +381,39 @@ def test_a_flush_by_one_rank_alone_changes_nothing():
     opt.step()
     opt.flush()
     assert (ps[0] == 1.0).all() and opt.allreduce is None
+
+
+class Growing(Exchange):
+    """Its connections may replace the buffers of those before, so no rank may still be at an exchange."""
+
+    def __init__(self, *args):
+        super().__init__(*args)
+        assert here.met, "made while another rank may still read what this one sent"
+
+    def apply(self, blob):
+        super().apply(blob)
+        here.met = False
+
+
+def test_ranks_meet_before_an_exchange_is_made(monkeypatch):
+    """The messages of one exchange are read before the next one's connections are made: another layout, and another
+    optimizer on the same environment."""
+    monkeypatch.setattr(optimizer, "_make_allreduce", Growing)
+    monkeypatch.setattr(Env, "barrier", lambda self: (self.meet.wait(), setattr(here, "met", True)))
+
+    def program(env, rank):
+        ps, more = [parameter(3), parameter(400)], [parameter(5000)]
+        ps[1].requires_grad_(False)
+        opt = ComprexAdamW(ps, env, weight_decay=0.0)
+        give(ps, 1.0)
+        opt.step()
+        ps[1].requires_grad_(True)
+        give(ps, 1.0)
+        opt.step()
+        give(more, 1.0)
+        ComprexAdamW(more, env, weight_decay=0.0).step()
+        met = here.met
+        opt.step()
+        assert met is here.met is False  # (only then)
+
+    run_ranks(2, program)
