@@ -274,7 +274,8 @@ class ComprexAdamW(torch.optim.Optimizer):
         """The steps' counts where they live on the device, into the state (a saved state holds numbers)."""
         for part in getattr(self, "_parts", None) or ():
             for count, members in part.counts:
-                n = int(count)
+                with torch.cuda.stream(self.handle.stream):  # behind the steps, whatever is current here
+                    n = int(count)
                 for k in members:
                     self.state[part.params[k]]["step"] = n
 

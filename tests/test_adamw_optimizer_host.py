@@ -417,3 +417,24 @@ def test_ranks_meet_before_an_exchange_is_made(monkeypatch):
         assert met is here.met is False  # (only then)
 
     run_ranks(2, program)
+
+
+class OnStream(torch.Tensor):
+    """A tensor that is written on a stream: a look at its value waits for the one that is current."""
+
+    def __int__(self):
+        assert here.stream.cuda_stream == 5
+        return super().__int__()
+
+
+def test_counts_on_the_device_are_read_in_the_order_of_their_stream():
+    """state_dict on another stream than the steps ran on: the counts are read behind them."""
+    ps = [parameter(3)]
+    opt = ComprexAdamW(ps, Env(), skip_nonfinite=True)
+    with on_stream(Stream(5)):
+        give(ps, 1.0)
+        opt.step()
+    for part in opt._parts:
+        part.counts = [(count.as_subclass(OnStream), of) for count, of in part.counts]
+    with on_stream(Stream(6)):
+        assert opt.state_dict()["state"][0]["step"] == 1
