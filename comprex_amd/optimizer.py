@@ -300,6 +300,10 @@ class ComprexAdamW(torch.optim.Optimizer):
                 self.handle = Handle(stream)
             for x in self._parts + self._kinds:
                 x.set = None
+        if stream.cuda_stream != self.handle.stream.cuda_stream:  # what another stream's memory holds is used on this one
+            for t in [count for part in self._parts for count, _ in part.counts] + [self.blob]:
+                if t is not None:
+                    t.record_stream(stream)
         self.handle.set_stream(stream)
         for kind in self._kinds:
             if kind.set is None:

@@ -438,3 +438,23 @@ def test_counts_on_the_device_are_read_in_the_order_of_their_stream():
         part.counts = [(count.as_subclass(OnStream), of) for count, of in part.counts]
     with on_stream(Stream(6)):
         assert opt.state_dict()["state"][0]["step"] == 1
+
+
+def test_buffers_are_known_to_the_streams_that_use_them(monkeypatch):
+    """The vector and the counts are allocated on one stream; steps on another tell the allocator, which would hand
+    them out again as soon as they are let go of."""
+    used = []
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, s: used.append((self.data_ptr(), s.cuda_stream)))
+
+    def program(env, rank):
+        ps = [parameter(3)]
+        opt = ComprexAdamW(ps, env, skip_nonfinite=True)
+        for raw in (5, 5, 6):
+            with on_stream(Stream(raw)):
+                give(ps, 1.0)
+                opt.step()
+        mine = {(t.data_ptr(), 6) for t in (opt.blob, opt._parts[0].counts[0][0])}
+        env.barrier()
+        assert mine <= set(used) and len(used) == 4
+
+    run_ranks(2, program)
