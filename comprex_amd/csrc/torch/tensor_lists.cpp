@@ -63,22 +63,29 @@ PyObject* addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyLong_FromLong(code);
 }
 
-// unmoved(tensors, count, at): whether `tensors` are `count` tensors at the addresses that the uint64 at `at` say.
+// unmoved(tensors, count, at, sizes, type): whether `tensors` are `count` tensors at the addresses that the uint64 at `at`
+// say, contiguous, with the element counts that the int64 at `sizes` say and of that type (type_code); without the last
+// two the addresses alone count.  (Memory that was let go of may come back as another tensor's at the same address.)
 PyObject* unmoved(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 3) {
-        PyErr_SetString(PyExc_TypeError, "unmoved(tensors, count, at)");
+    if (n != 3 && n != 5) {
+        PyErr_SetString(PyExc_TypeError, "unmoved(tensors, count, at[, sizes, type])");
         return nullptr;
     }
     const long long count = PyLong_AsLongLong(args[1]);
     const unsigned long long at = PyLong_AsUnsignedLongLong(args[2]);
+    const unsigned long long counts = n == 5 ? PyLong_AsUnsignedLongLong(args[3]) : 0;
+    const long long type = n == 5 ? PyLong_AsLongLong(args[4]) : 0;
     if (PyErr_Occurred()) return nullptr;
+    const int64_t* sizes = reinterpret_cast<const int64_t*>(counts);
     const uint64_t* want = reinterpret_cast<const uint64_t*>(at);
     if (!PyList_Check(args[0]) || PyList_GET_SIZE(args[0]) != count) Py_RETURN_FALSE;
     try {
         for (Py_ssize_t k = 0; k < count; ++k) {
             PyObject* item = PyList_GET_ITEM(args[0], k);
-            if (!THPVariable_Check(item) || reinterpret_cast<uint64_t>(THPVariable_Unpack(item).const_data_ptr()) != want[k])
-                Py_RETURN_FALSE;
+            if (!THPVariable_Check(item)) Py_RETURN_FALSE;
+            const at::Tensor& t = THPVariable_Unpack(item);
+            if (reinterpret_cast<uint64_t>(t.const_data_ptr()) != want[k]) Py_RETURN_FALSE;
+            if (sizes && (t.numel() != sizes[k] || type_code(t.scalar_type()) != type || !t.is_contiguous())) Py_RETURN_FALSE;
         }
     } catch (const std::exception&) {
         Py_RETURN_FALSE;
@@ -89,7 +96,7 @@ PyObject* unmoved(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {{"addresses", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(addresses)), METH_FASTCALL,
                           "addresses(tensors, count, sizes, out, device) -> type or -1"},
                          {"unmoved", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(unmoved)), METH_FASTCALL,
-                          "unmoved(tensors, count, at) -> bool"},
+                          "unmoved(tensors, count, at[, sizes, type]) -> bool"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_lists", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -201,10 +201,11 @@ class AdamWSet(TensorSet):
         wanted = [("params", dtype, sizes), ("exp_avg", torch.float8_e4m3fn if small else f32, sizes),
                   ("exp_avg_sq", torch.uint8 if small else f32, sizes), ("masters", f32, sizes),
                   ("exp_avg_scales", f32, blocks), ("exp_avg_sq_scales", f32, blocks)]
-        self.kept, self._at = lists, []
+        self.kept, self._at, self._is = lists, [], []  # the lists; per list the addresses, the sizes and the type
         for got, (name, dt, ns) in zip(lists, wanted):
             if got is None:
                 self._at.append(None)
+                self._is.append(None)
                 continue
             if len(got) != len(sizes):
                 raise _invalid("%d %s for %d parameters", len(got), name, len(sizes), code=_lib.CX_ERR_SIZE_MISMATCH)
@@ -213,6 +214,7 @@ class AdamWSet(TensorSet):
                                              -1 if handle.device.index is None else handle.device.index) != _TYPE_CODES[dt]:
                 self._examine_list(got, ns, name, dt, handle.device, at)
             self._at.append(at)
+            self._is.append((at.buffer_info()[0], counts, counts.buffer_info()[0], _TYPE_CODES[dt]))
         self.state_bits = 8 if small else 32
         at = [None if a is None else a.buffer_info()[0] for a in self._at]
         self._make(handle, sizes, C.byref(_lib.AdamwState(_NUM[dtype], self.state_bits, at[0], at[3], at[1], at[2], at[4],
@@ -229,10 +231,11 @@ class AdamWSet(TensorSet):
             at[k] = t.data_ptr()
 
     def made_of(self, lists):
-        """Whether the set was made of these tensors where they are now: lists in __init__'s order."""
+        """Whether the set was made of these tensors as and where they are now: lists in __init__'s order."""
         same = _lib.tensor_lists().unmoved
-        return all(x is at is None or (x is not None and at is not None and same(x, len(at), at.buffer_info()[0]))
-                   for x, at in zip(lists, self._at))
+        return all(x is known is None or (x is not None and known is not None and
+                                          same(x, len(self.sizes), known[0], known[2], known[3]))
+                   for x, known in zip(lists, self._is))
 
     @classmethod
     def zeros8(cls, param):

@@ -114,7 +114,7 @@ class _Part:
     steps are counted on the device, a count for each number that the parameters begin with, and whose it is."""
 
     def __init__(self, group, params):
-        self.group, self.params, self.states = group, params, []
+        self.group, self.params, self.states, self.dtype = group, params, [], params[0].dtype
         self.set, self.counts = None, []
 
     def tensors(self, state):
@@ -252,6 +252,8 @@ class ComprexAdamW(torch.optim.Optimizer):
                 self._check(p)
                 if "exp_avg" not in self.state[p]:
                     self._new_state(p)
+                if p.dtype == torch.float32:
+                    self.state[p].pop("master", None)  # (of a type that it had before)
                 alike.setdefault((str(p.dtype), k, self._small(p)), []).append(p)
 
         def form(p):
@@ -310,7 +312,13 @@ class ComprexAdamW(torch.optim.Optimizer):
                 kind.set = TensorSet(self.handle, [p.numel() for p in kind.params])
         for part in self._parts:
             lists = part.tensors(self.state)
-            if part.set is None or not part.set.made_of(lists):
+            if part.set is not None and not part.set.made_of(lists):
+                if any(p.dtype != part.dtype for p in part.params):  # other parts then
+                    self._sync_counts()
+                    self._make_parts()
+                    return self._make_sets()
+                part.set = None
+            if part.set is None:
                 part.set = AdamWSet(self.handle, *lists)
                 if self.skip_nonfinite and not part.counts:
                     part.count_on(stream.device)

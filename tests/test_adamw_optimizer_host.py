@@ -458,3 +458,38 @@ def test_buffers_are_known_to_the_streams_that_use_them(monkeypatch):
         assert mine <= set(used) and len(used) == 4
 
     run_ranks(2, program)
+
+
+def at_the_same_place(t, dtype, shape=None):
+    """Another tensor where `t` lies: what an allocation may get when the memory of `t` was let go of."""
+    return t.detach().view(torch.uint8)[:t.numel() * torch.empty(0, dtype=dtype).element_size()].view(dtype)
+
+
+def test_a_set_is_made_of_its_tensors_types_and_sizes_too():
+    p, m, v = torch.zeros(12), torch.zeros(12), torch.zeros(12)
+    s = HostAdamWSet(HostHandle(Stream(0)), [p], [m], [v])
+    lists = lambda x=p: [[x], [m], [v], None, None, None]  # noqa: E731
+    assert s.made_of(lists()) and s.made_of(lists(p.view(3, 4)))
+    assert not s.made_of(lists(p.clone()))
+    assert not s.made_of(lists(at_the_same_place(p, torch.bfloat16)))
+    assert not s.made_of(lists(p[:11])) and not s.made_of(lists(p.view(3, 4).t()))
+    assert not s.made_of([[p], [m], [v], [m], None, None]) and not s.made_of([[p], [m], [v[:11]], None, None, None])
+
+
+def test_a_parameter_whose_type_changes_where_it_lies():
+    """Halved and moved onto the memory it had: another type, another set."""
+    ps = [parameter(300, 1.0), parameter(20)]
+    opt = ComprexAdamW(ps, Env(), weight_decay=0.0)
+    give(ps, 1.0)
+    opt.step()
+    was = opt._parts[0].set
+    room = ps[0].data
+    ps[0].data = at_the_same_place(room, torch.bfloat16)
+    ps[0].data.fill_(3.0)
+    assert ps[0].data_ptr() == room.data_ptr()
+    give(ps, 1.0)
+    opt.step()
+    assert [part.set.kept[0][0].dtype for part in opt._parts] == [torch.bfloat16, torch.float32]
+    assert was not in [part.set for part in opt._parts]
+    assert (ps[0] == 2.0).all() and (ps[1] == -2.0).all()
+    assert [s["step"] for s in opt.state_dict()["state"].values()] == [2, 2]
