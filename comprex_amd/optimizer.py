@@ -197,6 +197,14 @@ class ComprexAdamW(torch.optim.Optimizer):
         if not p.is_cuda or not p.is_contiguous() or p.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise ValueError("parameters are contiguous fp32, bf16 or fp16 tensors on a GPU")
 
+    @staticmethod
+    def _check_group(group):
+        """Refuses what the step does not do (torch's own optimizers save such groups)."""
+        if group.get("amsgrad") or group.get("maximize"):
+            raise ValueError("`amsgrad` and `maximize` are not supported.")
+        if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
+            raise ValueError("the weight decay is AdamW's: it does not go through the moments.")
+
     def set_compression_ratio(self, compression_ratio):
         self.compression_ratio = compression_ratio
         if self.allreduce is not None:
@@ -204,10 +212,17 @@ class ComprexAdamW(torch.optim.Optimizer):
 
     def add_param_group(self, group):
         super().add_param_group(group)
+        try:
+            self._check_group(self.param_groups[-1])
+        except ValueError:
+            del self.param_groups[-1]
+            raise
         self._sync_counts()
         self._parts = None
 
     def load_state_dict(self, state_dict):
+        for group in state_dict["param_groups"]:
+            self._check_group({**self.defaults, **group})
         super().load_state_dict(state_dict)
         # the base class casts a parameter's state to the parameter's type: taken once more as it was saved
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]

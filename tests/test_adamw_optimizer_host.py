@@ -493,3 +493,25 @@ def test_a_parameter_whose_type_changes_where_it_lies():
     assert was not in [part.set for part in opt._parts]
     assert (ps[0] == 2.0).all() and (ps[1] == -2.0).all()
     assert [s["step"] for s in opt.state_dict()["state"].values()] == [2, 2]
+
+
+@pytest.mark.parametrize("bad", [dict(amsgrad=True), dict(maximize=True), dict(decoupled_weight_decay=False, weight_decay=0.1)],
+                         ids=str)
+def test_groups_of_another_update_are_refused(bad):
+    """What a state of torch's own optimizers may ask for and this step does not do; nothing is taken over then."""
+    p = parameter(5, 1.0)
+    opt = ComprexAdamW([p], Env(), learning_rate=0.5)
+    give([p], 1.0)
+    opt.step()
+    saved = opt.state_dict()
+    theirs = dict(saved, param_groups=[dict(saved["param_groups"][0], lr=0.25, **bad)])
+    with pytest.raises(ValueError):
+        opt.load_state_dict(theirs)
+    assert opt.param_groups[0]["lr"] == 0.5
+    fine = dict(saved, param_groups=[dict(saved["param_groups"][0], lr=0.25, amsgrad=False, maximize=False,
+                                          decoupled_weight_decay=True, foreach=None)])
+    opt.load_state_dict(fine)
+    assert opt.param_groups[0]["lr"] == 0.25
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[parameter(3)], **bad))
+    assert len(opt.param_groups) == 1
