@@ -232,6 +232,9 @@ class ComprexAdamW(torch.optim.Optimizer):
                 self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
                                  for k, v in state_dict["state"][i].items()}
                 self.state[p]["step"] = int(self.state[p]["step"])  # (torch's own optimizers save a tensor)
+                for k in ("exp_avg", "exp_avg_sq"):  # (and moments of the parameter's type)
+                    if self.state[p][k].dtype in (torch.bfloat16, torch.float16):
+                        self.state[p][k] = self.state[p][k].float()
         self._parts = None
         if self.allreduce is not None:
             self.allreduce.reset()  # what it held back are moves of the run that ends here
@@ -249,8 +252,6 @@ class ComprexAdamW(torch.optim.Optimizer):
         else:
             state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
             state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
-        if self.master_weights and p.dtype != torch.float32:
-            state["master"] = p.detach().to(torch.float32)
 
     def _training(self):
         return [p.requires_grad for group in self.param_groups for p in group["params"]]
@@ -269,6 +270,8 @@ class ComprexAdamW(torch.optim.Optimizer):
                     self._new_state(p)
                 if p.dtype == torch.float32:
                     self.state[p].pop("master", None)  # (of a type that it had before)
+                elif self.master_weights and "master" not in self.state[p]:
+                    self.state[p]["master"] = p.detach().to(torch.float32)
                 alike.setdefault((str(p.dtype), k, self._small(p)), []).append(p)
 
         def form(p):

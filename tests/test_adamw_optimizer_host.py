@@ -515,3 +515,26 @@ def test_groups_of_another_update_are_refused(bad):
     with pytest.raises(ValueError):
         opt.add_param_group(dict(params=[parameter(3)], **bad))
     assert len(opt.param_groups) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_state_of_torchs_adamw_for_16_bit_parameters(dtype):
+    """Its moments have the parameters' type and there are no masters: taken in 32 bits, and masters are made."""
+    p = parameter(7, 1.5, dtype)
+    theirs = torch.optim.AdamW([p], lr=1e-2)
+    give([p], 0.5)
+    theirs.step()
+    q = parameter(7, 0.0, dtype)
+    opt = ComprexAdamW([q], Env())
+    opt.load_state_dict(theirs.state_dict())
+    with torch.no_grad():
+        q.copy_(p)   # a model is restored before or after its optimizer
+    give([q], 0.5)
+    opt.step()
+    s = opt.state[q]
+    assert s["step"] == 2 and s["exp_avg"].dtype == s["exp_avg_sq"].dtype == s["master"].dtype == torch.float32
+    assert torch.equal(s["exp_avg"], theirs.state[p]["exp_avg"].float()) and torch.equal(s["master"], p.float())
+    other = ComprexAdamW([q], Env(), master_weights=False)
+    other.load_state_dict(theirs.state_dict())
+    other.step()
+    assert "master" not in other.state[q]
