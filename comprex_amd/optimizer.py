@@ -106,6 +106,7 @@ class ComprexOptimizer(torch.optim.Optimizer):
 
 #: the exchange counts in 32-bit integers
 _MOST_EXCHANGED = (1 << 31) - 1
+_LARGEST = torch.finfo(torch.float32).max
 _STATE = ("exp_avg", "exp_avg_sq", "master", "exp_avg_scales", "exp_avg_sq_scales")  # an AdamWSet's lists
 
 
@@ -179,8 +180,6 @@ class ComprexAdamW(torch.optim.Optimizer):
             raise ValueError("`state_bits` must be 8 or 32.")
         if clip_norm is not None and not clip_norm > 0:
             raise ValueError("`clip_norm` must be above 0.")
-        if not all(0 <= b < 1 for b in betas):
-            raise ValueError("`betas` must be in [0, 1).")
         super().__init__(params, dict(lr=learning_rate, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         for group in self.param_groups:
             for p in group["params"]:
@@ -199,11 +198,19 @@ class ComprexAdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _check_group(group):
-        """Refuses what the step does not do (torch's own optimizers save such groups)."""
+        """Refuses what the step does not do (torch's own optimizers save such groups) or would refuse."""
         if group.get("amsgrad") or group.get("maximize"):
             raise ValueError("`amsgrad` and `maximize` are not supported.")
         if group["weight_decay"] and not group.get("decoupled_weight_decay", True):
             raise ValueError("the weight decay is AdamW's: it does not go through the moments.")
+        if not all(0 <= b < 1 for b in group["betas"]):
+            raise ValueError("`betas` must be in [0, 1).")
+        if not 1e-20 <= group["eps"] <= _LARGEST:
+            raise ValueError("`eps` must be finite and at least 1e-20.")
+        if not 0 <= group["weight_decay"] <= _LARGEST:
+            raise ValueError("`weight_decay` must be finite and not negative.")
+        if not isinstance(group["lr"], torch.Tensor) and not 0 <= group["lr"] <= _LARGEST:
+            raise ValueError("the learning rate must be finite and not negative.")
 
     def set_compression_ratio(self, compression_ratio):
         self.compression_ratio = compression_ratio
@@ -365,6 +372,8 @@ class ComprexAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        for group in self.param_groups:
+            self._check_group(group)  # before a count or a moment changes
         ranks = self.gaspi_env.get_ranks()
         stream = self._ready()
         if stream is None:

@@ -538,3 +538,21 @@ def test_a_state_of_torchs_adamw_for_16_bit_parameters(dtype):
     other.load_state_dict(theirs.state_dict())
     other.step()
     assert "master" not in other.state[q]
+
+
+def test_what_the_step_would_refuse_is_refused_before_anything_counts():
+    p, q = parameter(5), parameter(6)
+    for bad in (dict(eps=0.0), dict(eps=1e-21), dict(eps=float("inf")), dict(weight_decay=-0.1), dict(learning_rate=-1.0),
+                dict(betas=(0.9, 1.0)), dict(weight_decay=float("nan"))):
+        with pytest.raises(ValueError):
+            ComprexAdamW([p], Env(), **bad)
+    with pytest.raises(ValueError):
+        ComprexAdamW([dict(params=[p]), dict(params=[q], eps=0.0)], Env())
+    opt = ComprexAdamW([dict(params=[p]), dict(params=[q])], Env(), learning_rate=torch.tensor(0.5))
+    give([p, q], 1.0)
+    opt.step()
+    opt.param_groups[1]["eps"] = 0.0
+    with pytest.raises(ValueError):
+        opt.step()
+    opt.param_groups[1]["eps"] = 1e-8
+    assert (p == -1.0).all() and [s["step"] for s in opt.state_dict()["state"].values()] == [1, 1]
