@@ -455,11 +455,11 @@ class ComprexAdamW(torch.optim.Optimizer):
             self.handle.adamw_step(part.set, these, count, group["lr"], **how)
         if part.counts:
             return
-        counts = set()
-        for s, g in zip(part.states, grads):
-            if g is not None:
-                s["step"] = n = s["step"] + 1
-                counts.add(n)
-        for n in sorted(counts):  # one, unless some parameter went without a gradient before
+        stepped = [s for s, g in zip(part.states, grads) if g is not None]
+        counts = {s["step"] for s in stepped}  # one, unless some parameter went without a gradient before
+        for n in sorted(counts, reverse=True):
             these = checked if len(counts) == 1 else [g if s["step"] == n else None for s, g in zip(part.states, grads)]
-            self.handle.adamw_step(part.set, these, n, group["lr"], **how)
+            self.handle.adamw_step(part.set, these, n + 1, group["lr"], **how)
+            for s in stepped:
+                if s["step"] == n:
+                    s["step"] = n + 1

@@ -556,3 +556,20 @@ def test_what_the_step_would_refuse_is_refused_before_anything_counts():
         opt.step()
     opt.param_groups[1]["eps"] = 1e-8
     assert (p == -1.0).all() and [s["step"] for s in opt.state_dict()["state"].values()] == [1, 1]
+
+
+def test_a_step_that_is_refused_does_not_count(monkeypatch):
+    p = parameter(5)
+    opt = ComprexAdamW([p], Env())
+    give([p], 1.0)
+
+    def refuse(*args, **how):
+        raise RuntimeError("refused")
+
+    with monkeypatch.context() as m:
+        m.setattr(HostHandle, "adamw_step", refuse)
+        with pytest.raises(RuntimeError):
+            opt.step()
+    assert opt.state[p]["step"] == 0
+    opt.step()
+    assert opt.state[p]["step"] == 1
