@@ -57,13 +57,16 @@ __device__ __forceinline__ void moments(Vec<float, N> g, const AdamwArgs& a, Vec
     v = v * a.beta2 + g * g * a.rest2;
 }
 
-template <int N>
+// EXACT: square root and quotient correctly rounded.  With moments in 32 bits HBM is the bound either way (25.6 M fp32
+// weights 115.4 us, the hardware's root and reciprocal 115.5; 100 M bf16 weights with masters 454 and 460).  With moments
+// in 8 bits the instructions nearly are, and root and reciprocal are the hardware's, to one unit in the last place.
+template <int N, bool EXACT>
 __device__ __forceinline__ Vec<float, N> moves_of(Vec<float, N> m, Vec<float, N> v, const AdamwArgs& a, const AdamwRates& r) {
     Vec<float, N> x;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-        const float below = __builtin_fmaf(__builtin_amdgcn_sqrtf(v[k]), r.v_unit, a.eps);
-        x[k] = r.step * (m[k] * __builtin_amdgcn_rcpf(below));
+        const float below = __builtin_fmaf(EXACT ? __builtin_sqrtf(v[k]) : __builtin_amdgcn_sqrtf(v[k]), r.v_unit, a.eps);
+        x[k] = r.step * (EXACT ? m[k] / below : m[k] * __builtin_amdgcn_rcpf(below));
     }
     return x;
 }
@@ -99,7 +102,7 @@ __global__ __launch_bounds__(kBlock) void adamw32_kernel(Pieces ps, GradArgs ga,
         if constexpr (TO == kMasters) w = load_some<4, FULL>(pw + i, k);
         if constexpr (TO == kWeights) w = to_float<4>(load_some<4, FULL>(p + i, k));
         moments<4>(to_float<4>(gx) * f, a, m, v);
-        const Vec<float, 4> move = moves_of<4>(m, v, a, r);
+        const Vec<float, 4> move = moves_of<4, true>(m, v, a, r);
         store_some<4, FULL>(pm + i, m, k);
         store_some<4, FULL>(pv + i, v, k);
         if constexpr (TO == kMoves) return store_some<4, FULL>(pw + i, move, k);
@@ -311,7 +314,7 @@ __global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, 
         const int mine = FULL || blocks > 1 ? (threadIdx.x >> 5) & 1 : 0;
         Vec<float, 8> m = m_value(mc, global(sm)[mine]), v = v_value(vc, global(sv)[mine]);
         moments<8>(to_float<8>(gx) * f, a, m, v);
-        const Vec<float, 8> move = moves_of<8>(m, v, a, r);
+        const Vec<float, 8> move = moves_of<8, false>(m, v, a, r);
         if constexpr (TO != kMoves) w = moved<8>(w, move, r.decay);
         if constexpr (TO == kMoves) e.store(pw, move);
         if constexpr (TO == kMasters) e.store(pw, w);

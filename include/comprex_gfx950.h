@@ -372,8 +372,8 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
  * master where there is one and the parameter otherwise:
  *     m = beta1 m + (1 - beta1) g            v = beta2 v + (1 - beta2) g^2
  *     w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- * in 32 bits (the square root and the reciprocal to one unit in the last place; a v below 2^-126 counts as 0
- * under the root); the parameter is w rounded once, 8-bit states are m and v rounded after w took them.
+ * in 32 bits (where moments have 8 bits, the square root and the reciprocal are taken to one unit in the last place,
+ * and a v below 2^-126 counts as 0 under the root); the parameter is w rounded once, 8-bit states are m and v rounded after w took them.
  * lr and weight_decay are finite in fp32 and not negative, the betas in [0, 1), eps is finite in fp32 and at least
  * 1e-20 (CX_ERR_INVALID).
  * step >= 1 counts this step.  With d_step (device int) the count lives on the device: the call adds 1 to

@@ -807,3 +807,16 @@ def test_refusals_on_the_device():
     before = p.clone()
     h.synchronize()
     assert torch.equal(p, before)
+
+
+def test_second_moments_below_the_normal_range_count_under_the_root():
+    """g = 2^-60: v = 0.001 g^2 lies below 2^-126, and with an eps of 1e-20 the root of it is nearly all that the move is
+    divided by.  v is rounded to a multiple of 2^-149 (2^-20 of it, 2^-21 of its root); a dozen other roundings."""
+    D = device_module()
+    p, m, v = (torch.zeros(1030, device="cuda") for _ in range(3))
+    h = D.Handle()
+    s = D.AdamWSet(h, [p], [m], [v])
+    g = 2.0 ** -60
+    h.adamw_step(s, [torch.full((1030,), g, device="cuda")], 1, 1.0, eps=1e-20, weight_decay=0.0)
+    want = g / (g + 1e-20)
+    assert (np.abs(f64(p) + want) <= want * (2.0 ** -21 + 14 * U)).all()
