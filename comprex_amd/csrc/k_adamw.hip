@@ -346,7 +346,10 @@ __global__ __launch_bounds__(kBlock) void set_states_kernel(Pieces ps, const flo
     if (blocks <= 0) return;
     const long long from = c.t.flat + c.at, block = c.at / CX_STATE_BLOCK + wave * 2;
     const Eight<true, false> e(c.n);
-    store_states(e, e.load(m_in + from), e.load(v_in + from), static_cast<unsigned char*>(c.t.m) + c.at,
+    Vec<float, 8> v = e.load(v_in + from);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = v[k] <= 0.0f ? 0.0f : v[k];  // -0 has no code, and a square is not below it
+    store_states(e, e.load(m_in + from), v, static_cast<unsigned char*>(c.t.m) + c.at,
                  static_cast<unsigned char*>(c.t.v) + c.at, c.t.m_scale + block, c.t.v_scale + block, blocks);
 }
 

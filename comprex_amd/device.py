@@ -508,7 +508,7 @@ class Handle:
         return m, v
 
     def adamw_set_states(self, tensors, exp_avg, exp_avg_sq):
-        """Sets the 8-bit moments of an AdamWSet from flat fp32 vectors (exp_avg_sq: not below 0)."""
+        """Sets the 8-bit moments of an AdamWSet from flat fp32 vectors (an exp_avg_sq below 0 counts as 0)."""
         if exp_avg is None or exp_avg_sq is None:
             raise _invalid("needs the values of both moments")
         check(self.lib.cx_adamw_set_states(self._h, tensors._t, tensors._vector(exp_avg, torch.float32, "exp_avg").data_ptr(),

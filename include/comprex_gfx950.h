@@ -401,7 +401,7 @@ int cx_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, double scale
                    double weight_decay);
 
 /* The values that the 8-bit states of a set stand for, all tensors back to back (dt: CX_F32, CX_BF16 or
- * CX_F16), and back: states from values (fp32).  For checkpoints that hold 32 bits. */
+ * CX_F16), and back: states from values (fp32; an exp_avg_sq below 0 counts as 0).  For checkpoints that hold 32 bits. */
 int cx_adamw_states(cx_handle h, cx_tensors t, cx_dtype dt, void* d_exp_avg, void* d_exp_avg_sq);
 int cx_adamw_set_states(cx_handle h, cx_tensors t, const float* d_exp_avg, const float* d_exp_avg_sq);
 

@@ -820,3 +820,23 @@ def test_second_moments_below_the_normal_range_count_under_the_root():
     h.adamw_step(s, [torch.full((1030,), g, device="cuda")], 1, 1.0, eps=1e-20, weight_decay=0.0)
     want = g / (g + 1e-20)
     assert (np.abs(f64(p) + want) <= want * (2.0 ** -21 + 14 * U)).all()
+
+
+def test_8bit_states_from_second_moments_that_are_not_above_zero():
+    """-0, and what another format's rounding left below 0, are 0: not the block's largest."""
+    D = device_module()
+    n = 2 * BLOCK + 7
+    p = torch.zeros(n, device="cuda")
+    state = D.AdamWSet.zeros8(p)
+    h = D.Handle()
+    s = D.AdamWSet(h, [p], [state[0]], [state[1]], exp_avg_scales=[state[2]], exp_avg_sq_scales=[state[3]])
+    v = torch.ones(n, device="cuda")
+    v[3:n:5], v[4:n:5], v[0] = -0.0, -2.0, math.nan
+    h.adamw_set_states(s, torch.ones(n, device="cuda"), v)
+    got = h.adamw_states(s)[1]
+    fine = v > 0
+    # 1 is its block's largest: exact but for the three roundings of a code's value
+    assert (got[fine] - 1).abs().max() <= 3.01 * U and got[1:][~fine[1:]].count_nonzero() == 0
+    assert state[1][0] == 255 and (state[3] == 1).all()
+    h.adamw_set_states(s, torch.ones(n, device="cuda"), -v.nan_to_num(1.0).abs())
+    assert h.adamw_states(s)[1].count_nonzero() == 0 and state[3].count_nonzero() == 0
