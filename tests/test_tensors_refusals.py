@@ -1,6 +1,8 @@
 """What the operators over many tensors refuse before anything reaches a device: the checks of the Python
 front end on host tensors, and those of the C entry point that makes a set."""
 import ctypes as C
+import os
+import subprocess
 
 import pytest
 import torch
@@ -188,3 +190,12 @@ def test_set_states_needs_both_vectors():
     h.lib, h._h = None, None
     refused(_lib.CX_ERR_INVALID, h.adamw_set_states, host_set([4]), None, torch.zeros(4))
     refused(_lib.CX_ERR_INVALID, h.adamw_set_states, host_set([4]), torch.zeros(4), None)
+
+
+def test_the_library_is_built_without_torch():
+    """A program in C or C++ needs the library alone; where torch is, its module is built too."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "comprex_amd", "csrc")
+    for python, lists in (("false", False), ("python3", True), ("python3 -S", False)):
+        r = subprocess.run(["make", "-n", "-B", "-C", csrc, "PYTHON=" + python, "all"], capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0, r.stderr
+        assert "libcomprex_gfx950.so" in r.stdout and ("_tensor_lists.so" in r.stdout) == lists
