@@ -33,7 +33,8 @@ class AdamwArgs(C.Structure):
     """cx_adamw_args"""
     _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
                 ("weight_decay", C.c_double), ("scale", C.c_double), ("step", C.c_longlong), ("d_step", C.c_void_p),
-                ("d_lr", C.c_void_p), ("d_coefs", C.c_void_p), ("n_coefs", C.c_int), ("d_skip", C.c_void_p), ("d_moves", C.c_void_p)]
+                ("d_lr", C.c_void_p), ("d_coefs", C.c_void_p), ("n_coefs", C.c_int), ("d_skip", C.c_void_p), ("d_moves", C.c_void_p),
+                ("rounding_seed", C.c_ulonglong)]
 
 
 class ComprexError(RuntimeError):

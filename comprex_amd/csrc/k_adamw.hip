@@ -22,6 +22,7 @@ struct AdamwRates {
     float step;        // lr / (1 - beta1^t)
     float decay;       // lr * weight_decay
     float v_unit;      // 1 / sqrt(1 - beta2^t)
+    unsigned long long noise;  // key of the step's rounding, where that is stochastic
 };
 
 struct AdamwArgs {
@@ -34,8 +35,20 @@ struct AdamwArgs {
     float* moves;                                   // where the moves go, if not into the weights
 };
 
-__host__ __device__ inline AdamwRates rates_of(double lr, double beta1, double beta2, double weight_decay, double t) {
+// Mixes 64 bits: the output function of SplitMix64 (Steele, Lea, Flood, "Fast splittable pseudorandom number
+// generators", 2014).
+constexpr unsigned long long kGolden = 0x9E3779B97F4A7C15ull;
+__host__ __device__ inline unsigned long long mixed(unsigned long long z) {
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+
+__host__ __device__ inline AdamwRates rates_of(double lr, double beta1, double beta2, double weight_decay, long long step,
+                                               unsigned long long seed) {
     AdamwRates r;
+    const double t = (double)step;
+    r.noise = mixed(seed + (unsigned long long)step * kGolden);
     r.step = (float)(lr / (1.0 - pow(beta1, t)));
     r.decay = (float)(lr * weight_decay);
     r.v_unit = (float)(1.0 / sqrt(1.0 - pow(beta2, t)));
@@ -44,10 +57,10 @@ __host__ __device__ inline AdamwRates rates_of(double lr, double beta1, double b
 
 // The step's count on the device: one thread advances it and leaves the rates for the step's kernel.
 __global__ void rates_kernel(int* count, long long step, const float* d_lr, double lr, double beta1, double beta2,
-                             double weight_decay, const int* skip, AdamwRates* rates) {
+                             double weight_decay, unsigned long long seed, const int* skip, AdamwRates* rates) {
     if (skip && *skip) return;
     if (count) step = ++*count;
-    *rates = rates_of(d_lr ? (double)*d_lr : lr, beta1, beta2, weight_decay, (double)step);
+    *rates = rates_of(d_lr ? (double)*d_lr : lr, beta1, beta2, weight_decay, step, seed);
 }
 
 // The moments; g already has its factor.
@@ -169,6 +182,37 @@ constexpr float kTiny = 0x1p-100f;               // a block below is stored as z
 constexpr float kVUnit = 0x1.ep-96f;             // V lies here before its bits are cut: exponent field 31, fraction 7/8
 constexpr float kVBack = (float)(0x1p96 / 1.875);
 
+// Rounded to nearest, a moment loses every change below half a code step, 3 to 6 % of it, for good: with beta2 = 0.999
+// a second moment moves by 0.1 % a step, and falls or rises with its block's largest only.  Rounded stochastically, up
+// with the probability that the remainder has of a code step, it follows in expectation: its relative variance settles
+// near (code step) * (change a step) / (2 * 0.001) = 0.09 * 0.001 / 0.002, about 0.05.  The remainder is what lies below
+// the code's bits in the scaled fp32 value, 20 bits; 16 random bits are added to its upper 16, and half of their unit, so that
+// a value that roundings moved off its code by a few units in the last place stays on it.
+//
+// A wave's random words: a mix of the step's key and the wave's place in the set, the same for all lanes (scalar
+// instructions); one more mix for each lane; from there eight words, one for each element, each a bijection of the one
+// before, so that every element's is as evenly spread over the steps as the lane's.  Lower half for m, upper for v.  100 M bf16 weights take
+// 180 us with noise and 160 to nearest (186 with three shifts a word), where instructions are the bound; 25.6 M in fp32 69.
+struct Nearest {};
+struct Noise {
+    unsigned x[8];
+    __device__ __forceinline__ Noise(unsigned long long key, long long place) {
+        const unsigned long long z = mixed(key + (unsigned long long)place * kGolden);
+        unsigned s = (unsigned)z + (threadIdx.x & 63) * (unsigned)(kGolden >> 32);
+        s = (s ^ (s >> 16)) * ((unsigned)(z >> 32) | 1u);
+        s = (s ^ (s >> 15)) * 0x4C957F2Du;  // (the lower half of Knuth's multiplier for 64-bit congruences)
+        s ^= s >> 16;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            s += s << 9;
+            s ^= s >> 14;
+            x[k] = s;
+        }
+    }
+    __device__ __forceinline__ unsigned lower(int k) const { return ((x[k] << 4) & 0xffff0u) | 8u; }
+    __device__ __forceinline__ unsigned upper(int k) const { return ((x[k] >> 12) & 0xffff0u) | 8u; }
+};
+
 struct Codes { unsigned x[2]; };                 // eight of them
 using Bytes = Vec<unsigned char, 8>;
 
@@ -226,7 +270,7 @@ __device__ __forceinline__ Vec<float, 8> v_value(Codes c, float scale) {
     for (int k = 0; k < 8; ++k) x[k] = __uint_as_float(((c.x[k / 4] >> (8 * (k % 4))) & 255u) << 20);
     return x * kVBack * scale;
 }
-__device__ __forceinline__ Codes m_codes(Vec<float, 8> m, float inverse) {
+__device__ __forceinline__ Codes m_codes(Vec<float, 8> m, float inverse, Nearest) {
     m = m * inverse;
     Codes c;
 #pragma unroll
@@ -236,14 +280,29 @@ __device__ __forceinline__ Codes m_codes(Vec<float, 8> m, float inverse) {
     }
     return c;
 }
+// e4m3's exponent and fraction bits are those of the value after a scaling that puts its smallest normal number at
+// fp32's; code 126 is the largest, 127 what is not finite.
+__device__ __forceinline__ Codes m_codes(Vec<float, 8> m, float inverse, const Noise& noise) {
+    m = m * inverse * 0x1p-120f;
+    Codes c = {};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const unsigned u = __float_as_uint(m[k]), size = u & 0x7fffffffu;
+        const unsigned code = size < 0x7f800000u ? min((size + noise.lower(k)) >> 20, 126u) : 127u;
+        c.x[k / 4] |= ((u >> 24 & 128u) | code) << (8 * (k % 4));
+    }
+    return c;
+}
+__device__ __forceinline__ unsigned v_remainder(Nearest, int) { return 0x80000u; }
+__device__ __forceinline__ unsigned v_remainder(const Noise& noise, int k) { return noise.upper(k); }
 // The value's own exponent and upper fraction bits, after a scaling that leaves 5 bits of exponent: small
-// values run into the format's subnormals as they do into those of fp32.  Rounded to nearest.
-__device__ __forceinline__ Codes v_codes(Vec<float, 8> v, float inverse) {
+// values run into the format's subnormals as they do into those of fp32.
+template <typename R> __device__ __forceinline__ Codes v_codes(Vec<float, 8> v, float inverse, const R& rounding) {
     const Vec<float, 8> y = v * inverse * kVUnit;
     Codes c = {};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const unsigned code = min((__float_as_uint(y[k]) + 0x80000u) >> 20, 255u);  // above 255 only what is not finite
+        const unsigned code = min((__float_as_uint(y[k]) + v_remainder(rounding, k)) >> 20, 255u);  // above 255 only what is not finite
         c.x[k / 4] |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * (k % 4));   // above 0: never 0
     }
     return c;
@@ -255,9 +314,9 @@ __device__ __forceinline__ unsigned lane_of(unsigned x, int lane) {
 
 // Rounds the moments of the wave's two blocks and stores them: the codes and the blocks' scales, sm and sv being
 // those of the wave's first one; `blocks` of them exist.
-template <bool SPLIT, bool FULL>
+template <bool SPLIT, bool FULL, typename R>
 __device__ __forceinline__ void store_states(const Eight<SPLIT, FULL>& e, Vec<float, 8> m, Vec<float, 8> v, unsigned char* pm,
-                                             unsigned char* pv, float* sm, float* sv, int blocks) {
+                                             unsigned char* pv, float* sm, float* sv, int blocks, const R& rounding) {
     unsigned mt = lane_max(m), vt = lane_max(v);
     half_max(mt, vt);
     if (max(max(lane_of(mt, 31), lane_of(mt, 63)), max(lane_of(vt, 31), lane_of(vt, 63))) >= 0x7f800000u) {
@@ -274,7 +333,7 @@ __device__ __forceinline__ void store_states(const Eight<SPLIT, FULL>& e, Vec<fl
     const unsigned quotient = __float_as_uint(kept ? (of_v ? 1.0f : 448.0f) / top : 0.0f);
     const float m_inverse = __uint_as_float(second ? lane_of(quotient, 32) : lane_of(quotient, 0));
     const float v_inverse = __uint_as_float(second ? lane_of(quotient, 48) : lane_of(quotient, 16));
-    const Codes mc = m_codes(m, m_inverse), all = v_codes(v, v_inverse);
+    const Codes mc = m_codes(m, m_inverse, rounding), all = v_codes(v, v_inverse, rounding);
     const bool v_kept = v_inverse > 0.0f;
     const Codes vc = {v_kept ? all.x[0] : 0u, v_kept ? all.x[1] : 0u};
     e.store(pm, __builtin_bit_cast(Bytes, mc));
@@ -284,7 +343,7 @@ __device__ __forceinline__ void store_states(const Eight<SPLIT, FULL>& e, Vec<fl
         global(of_v ? sv : sm)[b] = kept ? (of_v ? top : top * (float)(1.0 / 448.0)) : 0.0f;
 }
 
-template <typename P, typename G, int TO>
+template <typename P, typename G, int TO, bool NOISE>
 __global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, AdamwArgs a) {
     const Piece c = piece_of<kWide>(ps);
     const G* g = grad_of<G>(c, ga);
@@ -319,7 +378,8 @@ __global__ __launch_bounds__(kBlock) void adamw8_kernel(Pieces ps, GradArgs ga, 
         if constexpr (TO == kMoves) e.store(pw, move);
         if constexpr (TO == kMasters) e.store(pw, w);
         if constexpr (TO != kMoves) e.store(p, from_float<P, 8>(w));
-        store_states(e, m, v, pm, pv, sm, sv, blocks);
+        if constexpr (NOISE) store_states(e, m, v, pm, pv, sm, sv, blocks, Noise(r.noise, c.t.flat + c.at + wave * 512));
+        else store_states(e, m, v, pm, pv, sm, sv, blocks, Nearest());
     });
 }
 
@@ -350,20 +410,23 @@ __global__ __launch_bounds__(kBlock) void set_states_kernel(Pieces ps, const flo
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = v[k] <= 0.0f ? 0.0f : v[k];  // -0 has no code, and a square is not below it
     store_states(e, e.load(m_in + from), v, static_cast<unsigned char*>(c.t.m) + c.at,
-                 static_cast<unsigned char*>(c.t.v) + c.at, c.t.m_scale + block, c.t.v_scale + block, blocks);
+                 static_cast<unsigned char*>(c.t.v) + c.at, c.t.m_scale + block, c.t.v_scale + block, blocks, Nearest());
 }
 
+enum Moments { k32, k8Nearest, k8Noise };
+
 template <typename P, typename G, int TO>
-void launch_step(hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
-    if (bits == 32) adamw32_kernel<P, G, TO><<<n, kBlock, 0, s>>>(ps, g, a);
-    else adamw8_kernel<P, G, TO><<<n, kBlock, 0, s>>>(ps, g, a);
+void launch_step(hipStream_t s, Moments of, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
+    if (of == k32) adamw32_kernel<P, G, TO><<<n, kBlock, 0, s>>>(ps, g, a);
+    else if (of == k8Nearest) adamw8_kernel<P, G, TO, false><<<n, kBlock, 0, s>>>(ps, g, a);
+    else adamw8_kernel<P, G, TO, true><<<n, kBlock, 0, s>>>(ps, g, a);
 }
 
 template <typename P, int TO>
-void launch_step_for(int grad_type, hipStream_t s, int bits, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
-    if (grad_type == CX_F32) launch_step<P, float, TO>(s, bits, n, ps, g, a);
-    else if (grad_type == CX_BF16) launch_step<P, __bf16, TO>(s, bits, n, ps, g, a);
-    else launch_step<P, _Float16, TO>(s, bits, n, ps, g, a);
+void launch_step_for(int grad_type, hipStream_t s, Moments of, int n, const Pieces& ps, const GradArgs& g, const AdamwArgs& a) {
+    if (grad_type == CX_F32) launch_step<P, float, TO>(s, of, n, ps, g, a);
+    else if (grad_type == CX_BF16) launch_step<P, __bf16, TO>(s, of, n, ps, g, a);
+    else launch_step<P, _Float16, TO>(s, of, n, ps, g, a);
 }
 
 }  // namespace
@@ -383,14 +446,14 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
     if (u->d_step || u->d_lr) {
         AdamwRates* rates = reinterpret_cast<AdamwRates*>(t->d_rates);
         rates_kernel<<<1, 1, 0, h->stream>>>(u->d_step, u->step, u->d_lr, u->lr, u->beta1, u->beta2, u->weight_decay,
-                                             u->d_skip, rates);
+                                             u->rounding_seed, u->d_skip, rates);
         CX_HIP(hipGetLastError());
         a.device_rates = rates;
     } else {
-        a.rates = rates_of(u->lr, u->beta1, u->beta2, u->weight_decay, (double)u->step);
+        a.rates = rates_of(u->lr, u->beta1, u->beta2, u->weight_decay, u->step, u->rounding_seed);
     }
     return for_grads(t, g, t->state_bits == 32 ? kFine : kWide, [&](const Pieces& ps, int n, const GradArgs& ga) -> int {
-        const int bits = t->state_bits;
+        const Moments bits = t->state_bits == 32 ? k32 : u->rounding_seed ? k8Noise : k8Nearest;
         hipStream_t s = h->stream;
         if (u->d_moves) launch_step_for<float, kMoves>(g->type, s, bits, n, ps, ga, a);  // (no weights: no type of theirs)
         else if (t->param_type == CX_F32) launch_step_for<float, kWeights>(g->type, s, bits, n, ps, ga, a);

@@ -472,13 +472,17 @@ class Handle:
         return out
 
     def adamw_step(self, tensors, grads, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, coefs=None, scale=1.0,
-                   skip=None, moves=None):
+                   skip=None, moves=None, seed=None):
         """One AdamW step on an AdamWSet with the gradients times coefs and scale (cx_adamw_step).  `grads`: a
         list (None: leave this tensor alone) or the flat vector; `step`: which step this is, from 1, or an int32
         device tensor that the call advances; `lr`: a number or an fp32 device tensor; `skip` (int32) other than
         0: nothing changes.  With `moves`, a flat fp32 vector, the moments take the step and what the weights would
         lose goes there, for an exchange between ranks and `adamw_apply` (a tensor without a gradient: its part is
-        left as it is; skipped: zeros)."""
+        left as it is; skipped: zeros).  `seed`, a number from 1 to 2^64 - 1: moments in 8 bits are rounded stochastically
+        with noise from it, the step's count and an element's place, and follow their gradients over many steps, which
+        moments rounded to nearest (None) do not."""
+        if seed is not None and not 0 < seed < 1 << 64:
+            raise _invalid("a seed is a number from 1 to 2^64 - 1, not %s", seed)
         g = tensors.gradients(grads)
         on_device = isinstance(step, torch.Tensor)
         d_lr = isinstance(lr, torch.Tensor)
@@ -487,7 +491,7 @@ class Handle:
             0.0 if d_lr else lr, betas[0], betas[1], eps, weight_decay, scale, 0 if on_device else step,
             tensors._one(step, torch.int32, "step") if on_device else None,
             tensors._one(lr, torch.float32, "lr") if d_lr else None, at, n, tensors._one(skip, torch.int32, "skip"),
-            None if moves is None else tensors._vector(moves, torch.float32, "moves").data_ptr())))
+            None if moves is None else tensors._vector(moves, torch.float32, "moves").data_ptr(), seed or 0)))
 
     def adamw_apply(self, tensors, moves, lr, weight_decay=0.01, scale=1.0):
         """The weights of an AdamWSet after `scale` times the flat vector of moves (adamw_step) and the decay:

@@ -116,7 +116,7 @@ class _Part:
 
     def __init__(self, group, params):
         self.group, self.params, self.states, self.dtype = group, params, [], params[0].dtype
-        self.set, self.counts = None, []
+        self.set, self.counts, self.seed = None, [], None
 
     def tensors(self, state):
         """params, exp_avg, exp_avg_sq, masters, scales of both: lists, or None."""
@@ -158,7 +158,8 @@ class ComprexAdamW(torch.optim.Optimizer):
     flat fp32 vector through the exchange and come back summed, and every weight takes a `1 / ranks` of its sum
     and its decay; one without a gradient here may have had one elsewhere.
 
-    state_bits 8: the moments of parameters of at least `min_8bit_size` elements take one byte each.
+    state_bits 8: the moments of parameters of at least `min_8bit_size` elements take one byte each, rounded
+    stochastically, with the same noise in a run that is repeated or goes on from a saved state.
     master_weights: bf16 and fp16 parameters get fp32 weights of which they are the rounded values.
     skip_nonfinite: a gradient with an infinity or NaN anywhere leaves its rank's moments and count as they are,
     and its weights too or, with several ranks, its part of the sum zero; decided on the device, where the steps
@@ -287,6 +288,10 @@ class ComprexAdamW(torch.optim.Optimizer):
         self._parts = [_Part(self.param_groups[k], list(params))
                        for (_, k, _), those in sorted(alike.items(), key=lambda x: x[0][0])  # a kind's follow one another
                        for _, params in itertools.groupby(those, form)]
+        at = 0
+        for part in self._parts:  # moments in 8 bits are rounded with noise of each parameter's place
+            part.seed = 1 + at if form(part.params[0])[0] else None
+            at += sum(p.numel() for p in part.params)
         by_type = {}
         for part in self._parts:
             by_type.setdefault(part.params[0].dtype, []).append(part)
@@ -445,7 +450,7 @@ class ComprexAdamW(torch.optim.Optimizer):
         """The step of a part's parameters that have a gradient (`checked`: the same, ready for the set)."""
         group = part.group
         how = dict(betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"], coefs=coef, skip=flag,
-                   moves=moves)
+                   moves=moves, seed=part.seed)
         for count, members in part.counts:
             these = checked
             if len(part.counts) > 1:
