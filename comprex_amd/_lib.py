@@ -33,8 +33,7 @@ class AdamwArgs(C.Structure):
     """cx_adamw_args"""
     _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
                 ("weight_decay", C.c_double), ("scale", C.c_double), ("step", C.c_longlong), ("d_step", C.c_void_p),
-                ("d_lr", C.c_void_p), ("d_coefs", C.c_void_p), ("n_coefs", C.c_int), ("d_skip", C.c_void_p), ("d_moves", C.c_void_p),
-                ("rounding_seed", C.c_ulonglong)]
+                ("d_lr", C.c_void_p), ("d_coefs", C.c_void_p), ("n_coefs", C.c_int), ("d_skip", C.c_void_p), ("d_moves", C.c_void_p)]
 
 
 class ComprexError(RuntimeError):
@@ -109,6 +108,7 @@ def lib():
         "cx_grad_norms": (i, [vp, vp, C.POINTER(Grads), C.c_double, C.c_double, i, vp, vp, vp]),
         "cx_pack": (i, [vp, vp, C.POINTER(Grads), vp, i, C.c_double, vp, vp]),
         "cx_adamw_step": (i, [vp, vp, C.POINTER(Grads), C.POINTER(AdamwArgs)]),
+        "cx_adamw_step_seeded": (i, [vp, vp, C.POINTER(Grads), C.POINTER(AdamwArgs), C.c_ulonglong]),
         "cx_adamw_apply": (i, [vp, vp, vp, C.c_double, C.c_double, vp, C.c_double]),
         "cx_adamw_states": (i, [vp, vp, i, vp, vp]),
         "cx_adamw_set_states": (i, [vp, vp, vp, vp]),

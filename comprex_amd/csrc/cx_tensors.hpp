@@ -218,7 +218,7 @@ int launch_grad_norms(cx_handle h, cx_tensors t, const cx_grads* g, double scale
                       float* d_norms, float* d_coefs, int* d_nonfinite);
 int launch_pack(cx_handle h, cx_tensors t, const cx_grads* g, const float* d_coefs, int n_coefs, float scale,
                 const int* d_skip, float* out);
-int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_args* a);
+int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_args* a, unsigned long long seed);
 int launch_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, float scale, double lr, const float* d_lr,
                        double weight_decay);
 int launch_adamw_states(cx_handle h, cx_tensors t, int dt, void* d_m, void* d_v);

@@ -431,7 +431,7 @@ void launch_step_for(int grad_type, hipStream_t s, Moments of, int n, const Piec
 
 }  // namespace
 
-int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_args* u) {
+int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_args* u, unsigned long long seed) {
     AdamwArgs a = {};
     a.beta1 = (float)u->beta1;
     a.rest1 = (float)(1.0 - u->beta1);
@@ -446,14 +446,14 @@ int launch_adamw(cx_handle h, cx_tensors t, const cx_grads* g, const cx_adamw_ar
     if (u->d_step || u->d_lr) {
         AdamwRates* rates = reinterpret_cast<AdamwRates*>(t->d_rates);
         rates_kernel<<<1, 1, 0, h->stream>>>(u->d_step, u->step, u->d_lr, u->lr, u->beta1, u->beta2, u->weight_decay,
-                                             u->rounding_seed, u->d_skip, rates);
+                                             seed, u->d_skip, rates);
         CX_HIP(hipGetLastError());
         a.device_rates = rates;
     } else {
-        a.rates = rates_of(u->lr, u->beta1, u->beta2, u->weight_decay, u->step, u->rounding_seed);
+        a.rates = rates_of(u->lr, u->beta1, u->beta2, u->weight_decay, u->step, seed);
     }
     return for_grads(t, g, t->state_bits == 32 ? kFine : kWide, [&](const Pieces& ps, int n, const GradArgs& ga) -> int {
-        const Moments bits = t->state_bits == 32 ? k32 : u->rounding_seed ? k8Noise : k8Nearest;
+        const Moments bits = t->state_bits == 32 ? k32 : seed ? k8Noise : k8Nearest;
         hipStream_t s = h->stream;
         if (u->d_moves) launch_step_for<float, kMoves>(g->type, s, bits, n, ps, ga, a);  // (no weights: no type of theirs)
         else if (t->param_type == CX_F32) launch_step_for<float, kWeights>(g->type, s, bits, n, ps, ga, a);

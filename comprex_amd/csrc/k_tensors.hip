@@ -450,6 +450,10 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
 }
 
 int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* a) {
+    return cx_adamw_step_seeded(h, t, grads, a, 0);
+}
+
+int cx_adamw_step_seeded(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* a, unsigned long long seed) {
     int rc = check_set(h, t, "cx_adamw_step");
     if (rc == CX_OK) rc = check_grads(t, grads, "cx_adamw_step");
     if (rc == CX_OK && !a) rc = fail(CX_ERR_INVALID, "cx_adamw_step: null arguments");
@@ -470,7 +474,7 @@ int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_ada
     if (!a->d_step && a->step < 1) return fail(CX_ERR_INVALID, "cx_adamw_step: steps count from 1");
     DeviceScope on(t->device);
     CX_HIP(on.error);
-    return launch_adamw(h, t, grads, a);
+    return launch_adamw(h, t, grads, a, seed);
 }
 
 int cx_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, double scale, double lr, const float* d_lr,

@@ -487,11 +487,11 @@ class Handle:
         on_device = isinstance(step, torch.Tensor)
         d_lr = isinstance(lr, torch.Tensor)
         at, n = tensors._coefs(coefs)
-        check(self.lib.cx_adamw_step(self._h, tensors._t, g, _lib.AdamwArgs(
+        check(self.lib.cx_adamw_step_seeded(self._h, tensors._t, g, _lib.AdamwArgs(
             0.0 if d_lr else lr, betas[0], betas[1], eps, weight_decay, scale, 0 if on_device else step,
             tensors._one(step, torch.int32, "step") if on_device else None,
             tensors._one(lr, torch.float32, "lr") if d_lr else None, at, n, tensors._one(skip, torch.int32, "skip"),
-            None if moves is None else tensors._vector(moves, torch.float32, "moves").data_ptr(), seed or 0)))
+            None if moves is None else tensors._vector(moves, torch.float32, "moves").data_ptr()), seed or 0))
 
     def adamw_apply(self, tensors, moves, lr, weight_decay=0.01, scale=1.0):
         """The weights of an AdamWSet after `scale` times the flat vector of moves (adamw_step) and the decay:

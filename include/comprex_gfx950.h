@@ -319,7 +319,7 @@ typedef struct cx_tensors_s* cx_tensors;
  * block's largest |m|, scale M / 448.  exp_avg_sq: floats of 5 exponent and 3 mantissa bits without a sign
  * (code 8 e + f stands for 2^(e-1) (1 + f/8), for f / 8 where e = 0), in units that give the block's
  * largest value V the code 255, scale V; a value above 0 never becomes code 0.  Both are rounded to
- * nearest, or stochastically (cx_adamw_args.rounding_seed).  A block whose M (or V) is below 2^-100 is stored as zeros with scale 0.  Elements that are not
+ * nearest, or stochastically (cx_adamw_step_seeded).  A block whose M (or V) is below 2^-100 is stored as zeros with scale 0.  Elements that are not
  * finite count in no maximum and leave their block's others alone: their exp_avg is stored as NaN, such an
  * exp_avg_sq as the block's largest.
  * Bytes and scales that are zero stand for zero moments: how training begins. */
@@ -378,8 +378,9 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
  * 1e-20 (CX_ERR_INVALID).
  * Rounded to nearest, 8-bit moments hold for one step, not over many: a change below half a code step, 3 to 6 % of a
  * moment, is lost, and with beta2 = 0.999 v changes by 0.1 % a step, so it rises and falls with its block's largest
- * only.  rounding_seed != 0 rounds both moments stochastically, so that they follow the recurrences above in expectation
- * (v with a relative variance of about 0.05): what training takes.  The same seed, step and set give the same bits.
+ * only.  cx_adamw_step_seeded rounds both moments stochastically where the seed is not 0, so that they follow the recurrences
+ * above in expectation (v with a relative variance of about 0.05): what training takes.  The same seed, step and set give
+ * the same bits.
  * step >= 1 counts this step.  With d_step (device int) the count lives on the device: the call adds 1 to
  * it and uses the result; `step` is ignored.  d_lr (device float) replaces lr.  *d_skip != 0 leaves
  * everything as it is, *d_step too.
@@ -399,9 +400,9 @@ typedef struct {
     int n_coefs;               /* 0, 1 or the set's count */
     const int* d_skip;
     float* d_moves;
-    unsigned long long rounding_seed;   /* of 8-bit moments; 0: rounded to nearest */
 } cx_adamw_args;
 int cx_adamw_step(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* args);
+int cx_adamw_step_seeded(cx_handle h, cx_tensors t, const cx_grads* grads, const cx_adamw_args* args, unsigned long long seed);
 int cx_adamw_apply(cx_handle h, cx_tensors t, const float* d_moves, double scale, double lr, const float* d_lr,
                    double weight_decay);
 
