@@ -298,11 +298,11 @@ __device__ __forceinline__ unsigned v_remainder(const Noise& noise, int k) { ret
 // The value's own exponent and upper fraction bits, after a scaling that leaves 5 bits of exponent: small
 // values run into the format's subnormals as they do into those of fp32.
 template <typename R> __device__ __forceinline__ Codes v_codes(Vec<float, 8> v, float inverse, const R& rounding) {
-    const Vec<float, 8> y = v * inverse * kVUnit;
     Codes c = {};
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-        const unsigned code = min((__float_as_uint(y[k]) + v_remainder(rounding, k)) >> 20, 255u);  // above 255 only what is not finite
+        const float y = __builtin_fabsf(v[k]) * inverse * kVUnit;  // (a NaN's sign would leave no room for the remainder)
+        const unsigned code = min((__float_as_uint(y) + v_remainder(rounding, k)) >> 20, 255u);  // above 255 only what is not finite
         c.x[k / 4] |= max(code, min(__float_as_uint(v[k]), 1u)) << (8 * (k % 4));   // above 0: never 0
     }
     return c;

@@ -205,3 +205,24 @@ def test_seeds_that_are_none():
             S.h.adamw_step(S.set, g, 1, 1e-3, seed=seed)
     S.h.adamw_step(S.set, g, 1, 1e-3, seed=(1 << 64) - 1)
     assert np.isfinite(S.values()[0].cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("seed", [None, 3])
+@pytest.mark.parametrize("dtype,bits", [(F32, 0x7fc00000), (F32, 0xffc00000), (F32, 0x7fffffff), (F32, 0xffffffff), (F32, 0xff800001),
+                                        (BF16, 0xffff), (BF16, 0x7fff), (F16, 0xffff), (F16, 0xfe00)], ids=str)
+def test_every_nan_is_stored_as_the_blocks_largest(dtype, bits, seed):
+    """Whatever its sign and payload: exp_avg NaN, exp_avg_sq code 255, and the others as they are without it."""
+    S, T = Small([600]), Small([600])
+    g = torch.ones(600, dtype=dtype, device="cuda")
+    g[1::2] = 0.25
+    bad = g.clone()
+    word = torch.int32 if dtype == F32 else torch.int16
+    width = 8 * dtype.itemsize
+    bad.view(word)[5] = bits - (1 << width) if bits >> (width - 1) else bits
+    assert torch.isnan(bad[5])
+    S.h.adamw_step(S.set, [bad], 1, 0.0, seed=seed)
+    T.h.adamw_step(T.set, [g], 1, 0.0, seed=seed)
+    (m, v), (m0, v0) = S.values(), T.values()
+    assert torch.isnan(m[5]) and S.states[0][1][5] == 255
+    m[5], v[5] = m0[5], v0[5]
+    assert torch.equal(m, m0) and torch.equal(v, v0)
