@@ -380,7 +380,7 @@ int cx_pack(cx_handle h, cx_tensors t, const cx_grads* grads, const float* d_coe
  * moment, is lost, and with beta2 = 0.999 v changes by 0.1 % a step, so it rises and falls with its block's largest
  * only.  cx_adamw_step_seeded rounds both moments stochastically where the seed is not 0, so that they follow the recurrences
  * above in expectation (v with a relative variance of about 0.05): what training takes.  The same seed, step and set give
- * the same bits.
+ * the same bits; a captured step takes its count from d_step, so that replays round with noise of their own.
  * step >= 1 counts this step.  With d_step (device int) the count lives on the device: the call adds 1 to
  * it and uses the result; `step` is ignored.  d_lr (device float) replaces lr.  *d_skip != 0 leaves
  * everything as it is, *d_step too.

@@ -226,3 +226,39 @@ def test_every_nan_is_stored_as_the_blocks_largest(dtype, bits, seed):
     assert torch.isnan(m[5]) and S.states[0][1][5] == 255
     m[5], v[5] = m0[5], v0[5]
     assert torch.equal(m, m0) and torch.equal(v, v0)
+
+
+@pytest.mark.parametrize("moves", [False, True])
+def test_a_captured_step_rounds_with_each_replays_count(moves):
+    """A step with its count on the device, captured and replayed, has the bits of the eager steps 1, 2, ..."""
+    from comprex_amd import device as D
+    sizes = [3000, 5, 513]
+    A, B = Small(sizes, BF16, True), Small(sizes, BF16, True)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        B.h = D.Handle(side)
+        fixed = [torch.zeros(n, dtype=BF16, device="cuda") for n in sizes]
+        count = torch.zeros(1, dtype=torch.int32, device="cuda")
+
+    def step(S, grads, at):
+        S.h.adamw_step(S.set, grads, at, 1e-3, seed=9, moves=S.moves if moves else None)
+        if moves:
+            S.h.adamw_apply(S.set, S.moves, 1e-3)
+
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step(B, fixed, count)
+    torch.cuda.synchronize()
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for k in range(1, 7):
+        grads = [torch.empty(n, device="cuda").normal_(generator=gen).to(BF16) for n in sizes]
+        step(A, grads, k)
+        for f, g in zip(fixed, grads):
+            f.copy_(g)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert count.item() == k
+        assert all(torch.equal(p, q) for p, q in zip(A.p, B.p))
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for s, t in zip(A.states, B.states) for x, y in zip(s, t))

@@ -453,3 +453,99 @@ def test_refusals():
     p.grad = torch.sparse_coo_tensor(torch.tensor([[1]]), torch.tensor([1.0]), (10,)).cuda()
     with pytest.raises(RuntimeError):
         opt.step()
+
+
+def recording(monkeypatch):
+    """Every exchange keeps what it was given, by the thread and the exchange: {(thread, exchange): [vector, ...]}."""
+    from comprex_amd import optimizer
+    make, given = optimizer._make_allreduce, {}
+
+    def made(*args):
+        exchange = make(*args)
+        apply = exchange.apply
+
+        def recorded(vector):
+            given.setdefault((threading.get_ident(), id(exchange)), []).append(vector.clone())
+            return apply(vector)
+
+        exchange.apply = recorded
+        return exchange
+
+    monkeypatch.setattr(optimizer, "_make_allreduce", made)
+    return given
+
+
+def check_sums(got, w0, vectors, where, steps, R):
+    """Weights w0 less an R-th of the sum of all ranks' vectors.  With A the sum of their sizes: fewer than 2 steps R additions
+    on the way, and for each of steps + 1 updates of a weight a product and a difference."""
+    total = sum(f64(v) for v in vectors)
+    size = sum(np.abs(f64(v)) for v in vectors)
+    tol = (2 * steps * R * size / R + 2 * (steps + 2) * (np.abs(w0) + size / R)) * U
+    off = np.abs(got - (w0.astype(np.float64) - total / R))
+    assert (off <= tol)[where].all(), off[where].max()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("schedule", ["comprex_alltoone", "comprex_ring", "comprex_bigring"])
+def test_what_ranks_put_into_the_exchange_arrives(schedule, bits, monkeypatch):
+    """Two optimizers on streams of their own share an environment, three ranks.  After a flush the weights are w0 less a
+    third of all that the ranks put in: with the big ring on every rank, with all-to-one on the chief, with the ring (whose
+    broadcast drops what it does not send) on the rank where a segment's sum is made."""
+    R, steps, sizes = 3, 4, [[(70, 60), (5,), (300,)], [(5000,), (33, 3)]]
+    rng = np.random.default_rng(12)
+    totals = [sum(int(np.prod(s)) for s in of) for of in sizes]
+    w0 = [rng.standard_normal(n).astype(np.float32) for n in totals]
+    grads = [rng.standard_normal((R, steps, n)).astype(np.float32) for n in totals]
+    given, got, who = recording(monkeypatch), {}, {}
+
+    def program(env, rank):
+        who[threading.get_ident()] = rank
+        runs = []
+        for of, w in zip(sizes, w0):
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                params, at = [], 0
+                for s in of:
+                    k = int(np.prod(s))
+                    params.append(parameter(w[at:at + k].reshape(s)))
+                    at += k
+                runs.append((stream, params, ComprexAdamW(params, env, learning_rate=1e-2, weight_decay=0.0, state_bits=bits,
+                                                          allreduce_type=schedule, compression_ratio=0.05, size_factor=3.0)))
+        for step in range(steps):
+            for k, (stream, params, opt) in enumerate(runs):
+                with torch.cuda.stream(stream):
+                    at = 0
+                    for p in params:
+                        p.grad = torch.from_numpy(grads[k][rank, step, at:at + p.numel()]).cuda().view_as(p)
+                        at += p.numel()
+                    opt.step()
+        for k, (stream, params, opt) in enumerate(runs):
+            with torch.cuda.stream(stream):
+                opt.flush()
+            stream.synchronize()
+            # in the vector's order: moments in 8 bits and in 32 lie apart
+            order = [p for part in opt._parts for p in part.params]
+            start = torch.cat([torch.from_numpy(w).cuda() for w in np.split(w0[k], np.cumsum([p.numel() for p in params])[:-1])])
+            places = {id(p): x for p, x in zip(params, start.split([p.numel() for p in params]))}
+            got[k, rank] = (np.concatenate([f64(p).reshape(-1) for p in order]),
+                            np.concatenate([f64(places[id(p)]) for p in order]), id(opt.allreduce))
+        env.barrier()
+        for _, _, opt in runs:
+            opt.allreduce.apply = None  # (the wrapper keeps its exchange alive)
+
+    run_ranks(R, program)
+    for k, n in enumerate(totals):
+        vectors = [v for (thread, exchange), those in given.items() for v in those if exchange == got[k, who[thread]][2]]
+        assert len(vectors) == R * steps
+        segments = [n // R + (i < n % R) for i in range(R)]
+        starts = np.cumsum([0] + segments)
+        for rank in range(R):
+            where = np.zeros(n, bool)
+            if schedule == "comprex_bigring" or (schedule == "comprex_alltoone" and rank == 0):
+                where[:] = True
+            if schedule == "comprex_ring":
+                mine = (rank + 1) % R
+                where[starts[mine]:starts[mine + 1]] = True
+            weights, start, _ = got[k, rank]
+            check_sums(weights, start, vectors, where, steps, R)
+            assert np.isfinite(weights).all()
