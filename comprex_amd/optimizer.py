@@ -85,6 +85,8 @@ class ComprexOptimizer(torch.optim.Optimizer):
             return
         total = sum(p.numel() for p, _, _ in entries)
         if self.blob is None or self.blob.numel() != total:
+            # a channel grows for a larger vector: what an exchange before this one sent has to be read by then
+            self.gaspi_env.barrier()
             self.blob = torch.empty(total, dtype=torch.float32, device=entries[0][0].device)
             self.allreduce = self._create_allreduce(total)
         off = 0
@@ -405,8 +407,7 @@ class ComprexAdamW(torch.optim.Optimizer):
         if total == 0:
             return loss
         if self.blob is None:
-            # a channel grows for a larger vector: what an exchange before this one sent has to be read by then
-            self.gaspi_env.barrier()
+            self.gaspi_env.barrier()  # as in ComprexOptimizer.step
             self.blob = torch.empty(total, dtype=torch.float32, device=stream.device)
             self.allreduce = _make_allreduce(self.allreduce_type, self.gaspi_env, total, self.compression_ratio,
                                              self.size_factor)

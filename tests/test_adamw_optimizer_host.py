@@ -573,3 +573,23 @@ def test_a_step_that_is_refused_does_not_count(monkeypatch):
     assert opt.state[p]["step"] == 0
     opt.step()
     assert opt.state[p]["step"] == 1
+
+
+def test_ranks_meet_before_the_momentum_optimizer_makes_an_exchange(monkeypatch):
+    monkeypatch.setattr(optimizer, "_make_allreduce", Growing)
+    monkeypatch.setattr(Growing, "joined", lambda self: None)  # (it leaves the user stream to the program)
+    monkeypatch.setattr(Env, "barrier", lambda self: (self.meet.wait(), setattr(here, "met", True)))
+
+    def program(env, rank):
+        ps = [parameter(3), parameter(400)]
+        opt = optimizer.ComprexOptimizer(ps, env, learning_rate=1.0, momentum=0.0)
+        give(ps[:1], 1.0)
+        opt.step()
+        give(ps, 0.125)
+        opt.step()
+        met = here.met
+        opt.step()
+        assert met is here.met is False
+        assert (ps[0] == -1.25).all() and (ps[1] == -0.25).all()
+
+    run_ranks(2, program)
