@@ -191,9 +191,9 @@ constexpr float kVBack = (float)(0x1p96 / 1.875);
 //
 // A wave's random words: a mix of the step's key and the wave's place in the set, the same for all lanes (scalar
 // instructions); one more mix for each lane; from there eight words, one for each element, each a bijection of the one
-// before, so that every element's is as evenly spread over the steps as the lane's.  Lower half for m, upper for v.  100 M bf16 weights take
-// 180 to 195 us with noise and 160 to nearest (six more with three shifts a word): instructions are the bound there.  25.6 M in
-// fp32 take 69 us either way.
+// before, so that every element's is as evenly spread over the steps as the lane's.  Lower half for m, upper for v.
+// 100 M bf16 weights take 180 to 195 us with noise and 160 to nearest (six more with three shifts a word): instructions
+// are the bound there.  25.6 M in fp32 take 69 us either way.
 struct Nearest {};
 struct Noise {
     unsigned x[8];
